@@ -328,6 +328,104 @@ int qtb_attention_noalloc(const float *qkv, int batch, int n_heads, int n_kv, in
                           const int32_t *page_table, int pt_stride, const int32_t *pos,
                           int max_splits, float *out, void *stream);
 
+/* ---------------------------------------------------------------------------
+ * Operators of a serving step over a paged KV cache, on device memory.
+ *
+ * A step that mixes prompts, chunks of prompts and single-token decodes runs
+ * qtb_paged_plan once, then per layer qtb_paged_append and qtb_paged_attention
+ * (or qtb_prompt_attention, when every request starts from nothing and K and V
+ * are at hand).  They have no counterpart in the reference, whose cache is one
+ * request's contiguous rows.  Every pointer is DEVICE memory of the current
+ * device owned by the caller, `stream` a cudaStream_t (NULL = legacy default
+ * stream).  A call checks its arguments on the host, launches and returns: it
+ * never allocates, synchronises or keeps state, and may be captured into a
+ * graph.  Request lengths, page numbers and slots live on the device, so the
+ * kernels check them there: what is out of range is not accessed, and the
+ * reason is ORed into *status (NULL: not reported), which the caller zeroes.
+ * Every field is 64 bits wide; strides are in elements, the innermost
+ * dimension is contiguous, and tensor pointers and strides are multiples of 16
+ * bytes.  Nothing is read from tensors of extent zero. */
+enum {
+    QTB_T_F32 = 0,
+    QTB_T_BF16 = 1,
+    QTB_T_F16 = 2
+};
+enum {
+    QTB_PS_NO_PAGES = 1,    /* the free list ran out: table entry and slots -1       */
+    QTB_PS_ROW_FULL = 2,    /* a request outgrew its table row: its last slots -1    */
+    QTB_PS_ROOM = 4,        /* more than max_tokens new tokens: the rest is dropped  */
+    QTB_PS_LENGTH = 8,      /* a negative length: taken as 0                         */
+    QTB_PS_PAGE = 16        /* a page or slot outside the pool: read as zeros, not written */
+};
+
+/* Block tables and slot maps.  Request r has past_len[r] cached tokens in the
+ * pages table[r][0 .. ceil(past_len / page)) and brings new_len[r] tokens; the
+ * pages it needs beyond are taken from free_pages[*free_head ...] in request
+ * order and written to its row.  The new tokens are packed request by request:
+ * cu_new[r] is the first of request r, cu_new[n_req] their count. */
+typedef struct {
+    const int32_t *past_len, *new_len;   /* [n_req]                                */
+    int32_t *table;                      /* [n_req][table_stride], updated         */
+    const int32_t *free_pages;           /* [n_free] numbers of pages not in use   */
+    const int32_t *free_head;            /* first one to take, or NULL for 0       */
+    int32_t *cu_new;                     /* [n_req + 1]                            */
+    int32_t *kv_len;                     /* [n_req] past + new                     */
+    int64_t *slot;                       /* [max_tokens] page number * page + place, -1 behind the last token */
+    int32_t *pos, *req;                  /* [max_tokens] position and request, -1 likewise */
+    int32_t *free_head_out;              /* *free_head + pages taken (another word), or NULL */
+    int32_t *status;
+    int64_t n_req, max_tokens, table_cols, table_stride, n_free, page;
+} qtb_paged_plan_t;
+int qtb_paged_plan(const qtb_paged_plan_t *d, void *stream);
+
+/* Keys and values of n_tokens new tokens into the cache: position slot % page
+ * of page slot / page, every head, rounded to nearest even from f32.  Tokens
+ * whose slot is negative are skipped.  Two tokens never share a slot. */
+typedef struct {
+    const void *k, *v;                   /* [token][head][head_dim] of src_dtype   */
+    void *kpool, *vpool;                 /* [page][head][position][head_dim] of dtype */
+    const int64_t *slot;                 /* [n_tokens]                             */
+    int32_t *status;
+    int64_t k_stride[2], v_stride[2];    /* token, head                            */
+    int64_t kpool_stride[3], vpool_stride[3]; /* page, head, position              */
+    int64_t n_tokens, n_kv, head_dim, page, n_pages;
+    int64_t src_dtype, dtype;            /* dtype bf16 or f16; src_dtype the same or f32 */
+} qtb_paged_append_t;
+int qtb_paged_append(const qtb_paged_append_t *d, void *stream);
+
+/* Attention of each request's new tokens.  Query head h reads key head
+ * h / (n_heads / n_kv).  Paged form: K and V are pools [page][head][position]
+ * [head_dim], request r's keys 0 .. kv_len[r] - 1 lie in table[r], and its new
+ * tokens are its last ones (already appended).  Prompt form: K and V are packed
+ * like q ([token][head][head_dim]) and table, kv_len, page are not read.  A
+ * token at position p sees keys <= p (causal != 0) and > p - window (window >
+ * 0).  out = softmax(scale q.k) v in the type of q; lse = log sum exp(scale
+ * q.k), natural, f32 [n_tokens][n_heads] (NULL: not wanted).  A token that sees
+ * no key gets zeros and -inf.  head_dim 64 or 128; page a multiple of 16.
+ * max_new and max_kv bound new_len and kv_len over the requests: they choose
+ * how the work is split, not what is computed (0: not known). */
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    float *lse;
+    const int32_t *cu_new, *kv_len, *table;
+    int32_t *status;
+    void *workspace;                     /* qtb_attn_workspace bytes, 16-byte aligned */
+    int64_t workspace_bytes;
+    int64_t q_stride[2], out_stride[2];  /* token, head                            */
+    int64_t k_stride[3], v_stride[3];    /* paged: page, head, position; prompt: token, head */
+    int64_t table_stride, table_cols, page, n_pages;
+    int64_t n_req, n_tokens, n_heads, n_kv, head_dim;
+    int64_t max_new, max_kv;
+    int64_t dtype, causal, window;
+    double scale;
+} qtb_attn_t;
+/* Bytes of workspace for a call with these sizes (pointers are not read), or a
+ * negative QTB_E_* code.  Its contents matter during one call only. */
+int64_t qtb_attn_workspace(const qtb_attn_t *d);
+int qtb_paged_attention(const qtb_attn_t *d, void *stream);
+int qtb_prompt_attention(const qtb_attn_t *d, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -104,6 +104,15 @@ static int set_err(int code, const char *fmt, ...) {
   g_err = buf;
   return code;
 }
+// The same for the library's other translation units.
+int qtb_fail(int code, const char *fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return set_err(code, "%s", buf);
+}
 #define CUDA_TRY(call)                                                                          \
   do {                                                                                          \
     cudaError_t e_ = (call);                                                                    \
