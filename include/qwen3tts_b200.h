@@ -355,7 +355,8 @@ enum {
     QTB_PS_ROW_FULL = 2,    /* a request outgrew its table row: its last slots -1    */
     QTB_PS_ROOM = 4,        /* more than max_tokens new tokens: the rest is dropped  */
     QTB_PS_LENGTH = 8,      /* a negative length: taken as 0                         */
-    QTB_PS_PAGE = 16        /* a page or slot outside the pool: read as zeros, not written */
+    QTB_PS_PAGE = 16,       /* a page or slot outside the pool: read as zeros, not written */
+    QTB_PS_TIMEOUT = 32     /* a wait inside a kernel ran out: outputs are incomplete */
 };
 
 /* Block tables and slot maps.  Request r has past_len[r] cached tokens in the

@@ -1,0 +1,593 @@
+// qtb_attn_tile.cuh -- attention of many query rows on the 5th-generation
+// tensor cores.
+//
+// A query row is one (token, query head).  The rows of a request that share a
+// key head, token-major with the group's heads inside, fill tiles of 128 (as
+// many whole tokens as fit); a block works on two such tiles at a time, against
+// key tiles of 128, in two waves that hide each other:
+//
+//   load warp      Q tiles, then K_0 V_0 K_1 V_1 ... by TMA into a ring (128-byte
+//                  swizzle; a paged key tile is one box per run of a page's
+//                  positions)
+//   MMA warp       S = Q K^T into tensor memory, and O += P V with P from there;
+//                  tile 0's products run while tile 1's softmax does, and back
+//   warps 0-3, 4-7 softmax of tile 0, of tile 1: a thread has a row
+//   (warps 8 and 9 load and issue; 10 and 11 fill their warpgroup)
+//
+// Tensor memory (512 columns): S of both tiles (128 each; P, in the tensors'
+// type, takes S's place), O of both (head_dim each).
+//
+// The running maximum is renewed lazily: with scores in units of log2 (scale *
+// log2 e folded in), p = 2^(s - m) where m is a maximum seen so far, at most
+// 2^8 below the true one, so p <= 2^8 and the sum stays exact to f32 rounding;
+// only when a row outgrows that are its O and l scaled.  The final O / l does
+// not depend on m.
+//
+// Products are issued in order, so the commit that completes S of tile j also
+// says that P V of tile j - 1 is in O: the softmax warps may scale O then.
+// Every wait is bounded; one that runs out raises QTB_PS_TIMEOUT and all roles
+// leave.
+#pragma once
+#include "qtb_paged.cuh"
+#include <cuda.h>
+
+namespace qtb {
+
+constexpr int TILE_THREADS = 384, TILE_M = 128, TILE_N = 128;
+// Registers of a thread: the block starts with 168 for each of its 384 threads
+// (64512 in all); the softmax warps, a row of S each, take what the loading and
+// issuing warpgroup gives up: 256 * 200 + 128 * 96 = 63488.
+constexpr int TILE_REGS_SOFTMAX = 200, TILE_REGS_OTHER = 96;
+constexpr int TILE_SEGS = 256;             // entries of the in-block search over requests
+constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
+
+template <int HD>
+constexpr int tile_stages() { return HD == 128 ? 5 : 8; }
+template <int HD>
+constexpr int tile_kv_bytes() { return TILE_N * HD * 2; }
+template <int HD>
+constexpr int tile_smem() { return 1024 + 2 * TILE_M * HD * 2 + tile_stages<HD>() * tile_kv_bytes<HD>(); }
+
+struct TileMaps {
+  CUtensorMap q, k, v;
+};
+
+struct TileSync {
+  uint64_t q_full, q_empty, drain;
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t kv_full[8], kv_empty[8];
+  uint32_t tmem;
+  int abort;
+};
+
+// D (+)= A B with A in tensor memory.
+QTB_DEV void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of an operand whose N (or M) axis is contiguous: 64 elements of it
+// per 128-byte swizzled row, rows along K, 8-row groups 1024 bytes apart, the
+// next 64 elements `chunk` bytes further on.
+QTB_DEV uint64_t umma_desc_mn128(uint32_t saddr, uint32_t chunk) {
+  return (uint64_t)((saddr >> 4) & 0x3fffu) | ((uint64_t)((chunk >> 4) & 0x3fffu) << 16) |
+         ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+QTB_DEV void tmem_ld32_async(uint32_t taddr, float *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]),
+        "=f"(r[16]), "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]),
+        "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr));
+}
+QTB_DEV void tmem_ld16_async(uint32_t taddr, float *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      : "r"(taddr));
+}
+QTB_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+QTB_DEV void tmem_st16(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+QTB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+template <int N>
+QTB_DEV void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+QTB_DEV void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+QTB_DEV void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+QTB_DEV void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
+}
+QTB_DEV float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// One unit of work: 2 tpt tokens (a tile pair) of a request, one key head.
+struct TileItem {
+  AttnReq a;
+  int r, h, tok;        // request, key head, first token of the pair
+  int n_tok[2];         // tokens in each tile
+  int k0;               // first key of key tile 0 (a multiple of 128)
+  int n[2];             // key tiles of each query tile
+  int hi[2];            // keys at and past this are seen by no row of the tile
+};
+
+template <int HD, bool F16, bool PAGED>
+__global__ void __launch_bounds__(TILE_THREADS, 1)
+tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int box) {
+  constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
+  constexpr uint32_t S_COL = 0, O_COL = 256;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ TileSync sy;
+  __shared__ int s_pre[TILE_SEGS + 1];
+  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  unsigned char *s_q = smem, *s_kv = smem + 2 * Q_B;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tpt = TILE_M / c.group;        // tokens of a tile
+
+  // --- pairs of every request (those with more than row_limit rows), summed
+  const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS, n_seg = (c.n_req + seg - 1) / seg;
+  auto pairs_of = [&](int r) {
+    const int n = attn_request<PAGED>(c, r).n;
+    return n * c.group > row_limit ? (n + 2 * tpt - 1) / (2 * tpt) : 0;
+  };
+  for (int s = tid; s < TILE_SEGS; s += TILE_THREADS) {
+    int sum = 0;
+    if (s < n_seg)
+      for (int r = s * seg; r < min((s + 1) * seg, c.n_req); r++) sum += pairs_of(r);
+    s_pre[s] = sum;
+  }
+  if (tid == 0) {
+    mbar_init(&sy.q_full, 1); mbar_init(&sy.q_empty, 1); mbar_init(&sy.drain, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i], 128);
+      mbar_init(&sy.o_full[i], 1); mbar_init(&sy.o_empty[i], 128);
+    }
+    for (int i = 0; i < STAGES; i++) { mbar_init(&sy.kv_full[i], 1); mbar_init(&sy.kv_empty[i], 1); }
+    sy.abort = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (warp == 0) {                         // exclusive sums: a lane has 32 entries
+    int v[TILE_SEGS / 32], sum = 0;
+#pragma unroll
+    for (int i = 0; i < TILE_SEGS / 32; i++) { v[i] = s_pre[lane * (TILE_SEGS / 32) + i]; sum += v[i]; }
+    int pre = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, pre, o);
+      if (lane >= o) pre += x;
+    }
+    if (lane == 31) s_pre[TILE_SEGS] = pre;
+    pre -= sum;
+#pragma unroll
+    for (int i = 0; i < TILE_SEGS / 32; i++) { s_pre[lane * (TILE_SEGS / 32) + i] = pre; pre += v[i]; }
+  }
+  if (warp == 1) tmem_alloc(&sy.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = sy.tmem;
+  const int pairs = s_pre[TILE_SEGS];
+  const long long items = (long long)pairs * c.n_kv;
+
+  // Item i of the call, longest causal tiles first: pairs from the last to the
+  // first, key heads inside.  False past the end.
+  auto get_item = [&](long long i, TileItem &it) {
+    if (i >= items) return false;
+    it.h = (int)(i % c.n_kv);
+    int p = pairs - 1 - (int)(i / c.n_kv);
+    int lo = 0, hi = n_seg;                // s_pre[lo] <= p < s_pre[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s_pre[mid] <= p) lo = mid; else hi = mid;
+    }
+    p -= s_pre[lo];
+    it.r = lo * seg;
+    for (int q; p >= (q = pairs_of(it.r)); it.r++) p -= q;
+    it.a = attn_request<PAGED>(c, it.r);
+    it.tok = p * 2 * tpt;
+    const int left = it.a.n - it.tok;
+    it.n_tok[0] = min(left, tpt);
+    it.n_tok[1] = max(min(left - tpt, tpt), 0);
+    const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0;
+    it.k0 = low / TILE_N * TILE_N;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+      const int end = it.a.first + it.tok + t * tpt + it.n_tok[t];   // one past the tile's last token
+      it.hi[t] = c.causal ? min(end, it.a.hi) : it.a.hi;
+      it.n[t] = it.n_tok[t] > 0 && it.hi[t] > low ? (it.hi[t] - it.k0 + TILE_N - 1) / TILE_N : 0;
+    }
+    return true;
+  };
+  // Bounded wait of a whole warp; false: this or another role gave up.
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    bool ok = mbar_wait(bar, parity, 20000);
+    const long long t0 = clock64();
+    while (!ok && !*reinterpret_cast<volatile int *>(&sy.abort)) {
+      ok = mbar_wait(bar, parity, 20000);
+      if (!ok && clock64() - t0 > TILE_WAIT) {
+        *reinterpret_cast<volatile int *>(&sy.abort) = 1;
+        raise_status(c.status, QTB_PS_TIMEOUT);
+      }
+    }
+    return (bool)__all_sync(0xffffffffu, ok);
+  };
+
+  if (warp >= 8) {
+    regs_give<TILE_REGS_OTHER>();
+    if (warp == 8) {
+    // ------------------------------------------------------------- loads ---
+    int bad = 0;
+    uint32_t fill = 0, n_items = 0;        // ring fills issued; items begun
+    bool ok = true;
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      TileItem it;
+      if (!get_item(i, it)) break;
+      const int tiles = max(it.n[0], it.n[1]);
+      if (tiles == 0) continue;
+      const int hi = max(it.hi[0], it.hi[1]);
+      const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0;
+      auto load_q = [&]() {
+        if (!wait(&sy.q_empty, (n_items & 1) ^ 1)) return false;
+        if (lane == 0) {
+          const int rows = tpt * c.group, two = it.n_tok[1] > 0;
+          mbar_arrive_expect_tx(&sy.q_full, (uint32_t)(rows * 128 * (HD / 64) * (1 + two)));
+          for (int t = 0; t <= two; t++)
+            for (int x = 0; x < HD / 64; x++)
+              tma_load_4d(s_q + t * Q_B + x * HALF_B, &maps.q, x * 64, it.h * c.group, it.a.t0 + it.tok + t * tpt, 0, &sy.q_full);
+        }
+        n_items++;
+        return true;
+      };
+      for (int j = 0; j < tiles && ok; j++) {
+        const int kb = it.k0 + j * TILE_N;
+        // this lane's box of the key tile: positions [pos, pos + box), 64 dims
+        const int boxes = PAGED ? TILE_N / box : 1, bi = lane / (HD / 64), x = lane % (HD / 64);
+        const int pos = kb + bi * box;
+        const bool mine = bi < boxes && pos < hi && pos + box > low;
+        int pg = 0, off = 0;
+        if (PAGED && mine) {
+          const int e = pos / c.page;
+          off = pos - e * c.page;
+          pg = c.table[it.r * c.table_stride + e];
+          if (pg < 0 || pg >= c.n_pages) { pg = c.n_pages; bad |= QTB_PS_PAGE; }   // past the last page: reads zeros
+        }
+        const int count = __popc(__ballot_sync(0xffffffffu, mine));
+#pragma unroll
+        for (int kv = 0; kv < 2; kv++) {
+          const int st = (int)(fill % STAGES);
+          if (!wait(&sy.kv_empty[st], ((fill / STAGES) & 1) ^ 1)) { ok = false; break; }
+          if (lane == 0) mbar_arrive_expect_tx(&sy.kv_full[st], (uint32_t)(count * box * 128));
+          __syncwarp();
+          if (mine) {
+            unsigned char *dst = s_kv + st * KV_B + x * HALF_B + bi * box * 128;
+            const CUtensorMap *map = kv ? &maps.v : &maps.k;
+            if (PAGED) tma_load_4d(dst, map, x * 64, off, it.h, pg, &sy.kv_full[st]);
+            else tma_load_4d(dst, map, x * 64, it.a.t0 + pos, it.h, 0, &sy.kv_full[st]);
+          }
+          fill++;
+          // the queries' buffer may still serve the item before: its keys go first
+          if (kv == 0 && j == 0 && !load_q()) { ok = false; break; }
+        }
+      }
+    }
+    // copies in flight land before the block leaves
+    for (uint32_t f = fill > STAGES ? fill - STAGES : 0; f < fill; f++)
+      mbar_wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1, TILE_WAIT);
+    if (n_items) mbar_wait(&sy.q_full, (n_items - 1) & 1, TILE_WAIT);
+    raise_status(c.status, bad);
+    } else if (warp == 9) {
+    // --------------------------------------------------------------- MMA ---
+    const uint32_t ab = F16 ? 0u : 1u;
+    const uint32_t idesc_s = umma_idesc(1u, ab, TILE_N), idesc_o = umma_idesc(1u, ab, HD) | (1u << 16);   // B as [K][N]
+    uint32_t fill = 0, n_items = 0, p_n[2] = {0, 0}, o_n[2] = {0, 0};
+    bool ok = true, issued = false;
+    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+      TileItem it;
+      if (!get_item(i, it)) break;
+      const int tiles = max(it.n[0], it.n[1]);
+      if (tiles == 0) continue;
+      if (!wait(&sy.q_full, n_items & 1)) break;
+      n_items++;
+      auto scores = [&](int t, int st) {
+        if (lane == 0) {
+          const uint32_t q = smem_u32(s_q + t * Q_B), k = smem_u32(s_kv + st * KV_B);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ks++) {
+            const uint32_t o = (ks >> 2) * HALF_B + (ks & 3) * 32;
+            umma_bf16(tmem + S_COL + t * 128, umma_desc_sw128(q + o), umma_desc_sw128(k + o), idesc_s, ks != 0);
+          }
+          umma_commit(&sy.s_full[t]);
+        }
+        __syncwarp();
+      };
+      int st = (int)(fill % STAGES);
+      if (!(ok = wait(&sy.kv_full[st], (fill / STAGES) & 1))) break;
+      issued = true;
+      for (int t = 0; t < 2; t++)
+        if (it.n[t] > 0) scores(t, st);
+      if (lane == 0) {
+        umma_commit(&sy.kv_empty[st]);
+        if (tiles == 1) umma_commit(&sy.q_empty);
+      }
+      fill++;
+      for (int j = 0; j < tiles && ok; j++) {
+        const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
+        if (!(ok = wait(&sy.kv_full[sv], (fill / STAGES) & 1))) break;
+        if (j + 1 < tiles && !(ok = wait(&sy.kv_full[sk], ((fill + 1) / STAGES) & 1))) break;
+        for (int t = 0; t < 2 && ok; t++) {
+          if (j >= it.n[t]) continue;
+          if (j == 0 && !(ok = wait(&sy.o_empty[t], (o_n[t] & 1) ^ 1))) break;
+          if (!(ok = wait(&sy.p_full[t], p_n[t] & 1))) break;
+          p_n[t]++;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t v = smem_u32(s_kv + sv * KV_B);
+#pragma unroll
+            for (int ks = 0; ks < TILE_N / 16; ks++)
+              umma_ts(tmem + O_COL + t * HD, tmem + S_COL + t * 128 + ks * 8, umma_desc_mn128(v + ks * 2048, HALF_B), idesc_o,
+                      (j | ks) != 0);
+            if (j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
+          }
+          __syncwarp();
+          if (j == it.n[t] - 1) o_n[t]++;
+          if (j + 1 < it.n[t]) scores(t, sk);
+        }
+        if (!ok) break;
+        if (lane == 0) {
+          umma_commit(&sy.kv_empty[sv]);
+          if (j + 1 < tiles) umma_commit(&sy.kv_empty[sk]);
+          if (j + 2 == tiles) umma_commit(&sy.q_empty);
+        }
+        fill += j + 1 < tiles ? 2 : 1;
+      }
+    }
+    if (issued) {                          // nothing reads shared or tensor memory any more
+      if (lane == 0) umma_commit(&sy.drain);
+      __syncwarp();
+      mbar_wait(&sy.drain, 0, TILE_WAIT);
+    }
+    }
+  } else {
+    regs_take<TILE_REGS_SOFTMAX>();
+    // ----------------------------------------------------------- softmax ---
+    const int t = warp >> 2, row = tid & 127;
+    const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+    const uint32_t s_at = tmem + S_COL + t * 128 + lanes, o_at = tmem + O_COL + t * HD + lanes;
+    uint32_t fill = 0, s_n = 0, o_n = 0;
+    for (long long i = blockIdx.x;; i += gridDim.x) {
+      TileItem it;
+      if (!get_item(i, it)) break;
+      const int tiles = max(it.n[0], it.n[1]), n = it.n[t];
+      const int tt = row / c.group, tok = it.tok + t * tpt + tt, pos = it.a.first + tok;
+      const bool live = tt < it.n_tok[t];
+      const int last = min(c.causal ? pos : it.a.hi - 1, it.a.hi - 1);
+      const int first = c.window > 0 ? max(pos - c.window + 1, 0) : 0;
+      // what every row of the tile sees of a key tile lies within these
+      const int pos_a = it.a.first + it.tok + t * tpt, pos_b = pos_a + it.n_tok[t] - 1;
+      const int all_last = min(c.causal ? pos_a : it.a.hi - 1, it.a.hi - 1);
+      const int all_first = c.window > 0 ? max(pos_b - c.window + 1, 0) : 0;
+      const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0, high = max(it.hi[0], it.hi[1]);
+      float m = -INFINITY, l = 0.f;
+      bool ok = true;
+      for (int j = 0; j < n; j++) {
+        if (!(ok = wait(&sy.s_full[t], s_n & 1))) break;
+        s_n++;
+        tc_fence_after();
+        const int kb = it.k0 + j * TILE_N;
+        float s[128];
+#pragma unroll
+        for (int x = 0; x < 4; x++) tmem_ld32_async(s_at + 32 * x, s + 32 * x);
+        tmem_ld_wait();
+        if (kb + TILE_N - 1 > all_last || kb < all_first) {
+          const int a = first - kb, b = last - kb;
+#pragma unroll
+          for (int x = 0; x < 128; x++) s[x] = x >= a && x <= b ? s[x] : -INFINITY;
+        }
+        float mx[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) mx[x] = max3(s[x], s[x + 4], s[x + 8]);
+#pragma unroll
+        for (int x = 12; x + 8 <= 128; x += 8)
+#pragma unroll
+          for (int y = 0; y < 4; y++) mx[y] = max3(mx[y], s[x + y], s[x + 4 + y]);
+#pragma unroll
+        for (int y = 0; y < 4; y++) mx[y] = fmaxf(mx[y], s[124 + y]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c.scale_log2;
+        if (__any_sync(0xffffffffu, top > m + 8.f)) {
+          const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_approx(m - m2);
+          m = m2;
+          l *= f;
+          if (j > 0) {
+#pragma unroll 1
+            for (int x = 0; x < HD / 16; x++) {
+              float o[16];
+              uint32_t w[16];
+              tmem_ld16_async(o_at + 16 * x, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int y = 0; y < 16; y++) w[y] = __float_as_uint(o[y] * f);
+              tmem_st16(o_at + 16 * x, w);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int part = 0; part < 4; part++) {
+          // rounded to the tensors' type for the product with V, as large as
+          // the result's own rounding; the sum is of the unrounded ones
+          uint32_t p[16];
+#pragma unroll
+          for (int x = 0; x < 16; x++) {
+            const float a = exp2_approx(fmaf(s[32 * part + 2 * x], c.scale_log2, -base));
+            const float b = exp2_approx(fmaf(s[32 * part + 2 * x + 1], c.scale_log2, -base));
+            sum[x & 1] += a;
+            sum[2 + (x & 1)] += b;
+            p[x] = pack2<F16>(a, b);
+          }
+          tmem_st16(s_at + 16 * part, p);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (kb < low || kb + TILE_N > high) {
+          // keys that no row sees: their V may be anything, and 0 * NaN is NaN
+          const uint32_t f = fill + 2 * j + 1;
+          unsigned char *v = s_kv + (f % STAGES) * KV_B;
+          if (!(ok = wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1))) break;
+          if (kb + row < low || kb + row >= high) {
+#pragma unroll
+            for (int x = 0; x < HD / 64; x++)
+#pragma unroll
+              for (int y = 0; y < 8; y++)
+                *reinterpret_cast<uint4 *>(v + x * HALF_B + row * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&sy.p_full[t]);
+      }
+      if (!ok) break;
+      fill += 2 * tiles;
+      if (n > 0) {
+        if (!wait(&sy.o_full[t], o_n & 1)) break;
+        o_n++;
+        tc_fence_after();
+      }
+      const long long tk = it.a.t0 + tok;
+      const int h = it.h * c.group + row - tt * c.group;
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
+      uint16_t *op = c.out + tk * c.o_st + h * c.o_sh;
+#pragma unroll
+      for (int x = 0; x < HD / 32; x++) {
+        float o[32];
+        if (n > 0) {
+          tmem_ld32_async(o_at + 32 * x, o);
+          tmem_ld_wait();
+        }
+        if (live) {
+#pragma unroll
+          for (int y = 0; y < 4; y++) {
+            uint32_t w[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+              w[z] = n > 0 ? pack2<F16>(o[8 * y + 2 * z] * inv, o[8 * y + 2 * z + 1] * inv) : 0u;
+            *reinterpret_cast<uint4 *>(op + 32 * x + 8 * y) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        __syncwarp();
+      }
+      if (n > 0) {
+        tc_fence_before();
+        mbar_arrive(&sy.o_empty[t]);
+      }
+      if (live && c.lse) c.lse[tk * c.n_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------------ host ---
+typedef CUresult (*TileEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A tensor [d3][d2][d1][hd] (extents and strides of the outer axes, innermost
+// first) in boxes of [1][b2][b1][64] with the 128-byte swizzle.  False where TMA
+// cannot describe it (an expanded axis has stride 0).
+static inline bool tile_map(TileEncodeFn fn, CUtensorMap *out, const void *base, bool f16, int hd, const long long (&ext)[3],
+                            const long long (&st)[3], int b1, int b2) {
+  cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)ext[0], (cuuint64_t)ext[1], (cuuint64_t)ext[2]}, bytes[3];
+  for (int i = 0; i < 3; i++) {
+    if (ext[i] < 1 || (ext[i] > 1 && st[i] <= 0)) return false;
+    bytes[i] = ext[i] > 1 ? (cuuint64_t)st[i] * 2 : (cuuint64_t)hd * 2;   // of an axis of one, any stride will do
+  }
+  const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, one[4] = {1, 1, 1, 1};
+  return fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, bytes,
+            box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The key box: as many of a page's positions as divide both page and tile.
+static inline int tile_box(bool paged, int page) {
+  int b = TILE_N;
+  while (paged && page % b) b >>= 1;
+  return b;
+}
+
+// Whether the tensors have a form that the tile kernel reads, and its maps.
+static inline bool tile_maps(const AttnCall &c, bool paged, bool f16, int hd, TileEncodeFn fn, TileMaps &m) {
+  if (!fn || !(c.scale_log2 > 0.f)) return false;   // its maximum is taken before scaling
+  const int tpt = TILE_M / c.group, box = tile_box(paged, c.page);
+  const long long qe[3] = {c.n_heads, c.n_tokens, 1}, qs[3] = {c.q_sh, c.q_st, 0};
+  if (!tile_map(fn, &m.q, c.q, f16, hd, qe, qs, c.group, tpt)) return false;
+  if (paged) {
+    const long long e[3] = {c.page, c.n_kv, c.n_pages};
+    const long long ks[3] = {c.k_st[2], c.k_st[1], c.k_st[0]}, vs[3] = {c.v_st[2], c.v_st[1], c.v_st[0]};
+    return tile_map(fn, &m.k, c.k, f16, hd, e, ks, box, 1) && tile_map(fn, &m.v, c.v, f16, hd, e, vs, box, 1);
+  }
+  const long long e[3] = {c.n_tokens, c.n_kv, 1};
+  const long long ks[3] = {c.k_st[0], c.k_st[1], 0}, vs[3] = {c.v_st[0], c.v_st[1], 0};
+  return tile_map(fn, &m.k, c.k, f16, hd, e, ks, box, 1) && tile_map(fn, &m.v, c.v, f16, hd, e, vs, box, 1);
+}
+
+template <int HD, bool F16, bool PAGED>
+static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, int grid, int row_limit, cudaStream_t st) {
+  if (prepare)
+    return cudaFuncSetAttribute(tile_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<HD>());
+  tile_kernel<HD, F16, PAGED><<<grid, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tile_box(PAGED, c->page));
+  return cudaGetLastError();
+}
+static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int grid, int row_limit,
+                                   cudaStream_t st) {
+  switch (which) {
+    case 0: return tile_run<64, false, false>(prepare, c, m, grid, row_limit, st);
+    case 1: return tile_run<64, false, true>(prepare, c, m, grid, row_limit, st);
+    case 2: return tile_run<64, true, false>(prepare, c, m, grid, row_limit, st);
+    case 3: return tile_run<64, true, true>(prepare, c, m, grid, row_limit, st);
+    case 4: return tile_run<128, false, false>(prepare, c, m, grid, row_limit, st);
+    case 5: return tile_run<128, false, true>(prepare, c, m, grid, row_limit, st);
+    case 6: return tile_run<128, true, false>(prepare, c, m, grid, row_limit, st);
+    default: return tile_run<128, true, true>(prepare, c, m, grid, row_limit, st);
+  }
+}
+static inline cudaError_t tile_prepare() {
+  for (int i = 0; i < 8; i++)
+    if (cudaError_t e = tile_any(true, i, nullptr, nullptr, 0, 0, nullptr)) return e;
+  return cudaSuccess;
+}
+// Requests with more than row_limit query rows to a key head are served.
+static inline cudaError_t tile_launch(const AttnCall &c, bool paged, bool f16, int hd, const TileMaps &m, int sms, int row_limit,
+                                      cudaStream_t st) {
+  const int tpp = 2 * (TILE_M / c.group);
+  const long long pairs = c.n_req == 1 ? (c.n_tokens + tpp - 1) / tpp : c.n_tokens / tpp + c.n_req;   // at most
+  const long long items = pairs * c.n_kv;
+  return tile_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, (int)(items < sms ? items : sms),
+                  row_limit, st);
+}
+
+}  // namespace qtb

@@ -6,6 +6,7 @@
 // (qtb_prompt_attention).  No call allocates, synchronises or keeps state.
 #include "qtb_paged.cuh"
 #include "qtb_attn_rows.cuh"
+#include "qtb_attn_tile.cuh"
 
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -230,6 +231,7 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendCall c)
 constexpr int MAX_DEV = 64;
 struct DevInfo {
   int sms = 0;
+  TileEncodeFn encode = nullptr;           // cuTensorMapEncodeTiled
   cudaError_t err = cudaSuccess;
 };
 
@@ -249,6 +251,13 @@ int device_info(const DevInfo **out) {
     if (d.err == cudaSuccess && major != 10) d.err = cudaErrorNoKernelImageForDevice;
     if (d.err == cudaSuccess) d.err = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev);
     if (d.err == cudaSuccess) d.err = rows_prepare();
+    if (d.err == cudaSuccess) d.err = tile_prepare();
+    if (d.err == cudaSuccess) {
+      void *p = nullptr;
+      cudaDriverEntryPointQueryResult q;
+      d.err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
+      if (q == cudaDriverEntryPointSuccess) d.encode = reinterpret_cast<TileEncodeFn>(p);
+    }
   });
   if (d.err != cudaSuccess) return qtb_fail(QTB_E_CUDA, "paged operators on device %d: %s", dev, cudaGetErrorString(d.err));
   *out = &d;
@@ -315,8 +324,14 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   if (need < 0) return (int)need;
   if (d->workspace_bytes < need || (need && !d->workspace) || !aligned16(d->workspace))
     return qtb_fail(QTB_E_INVALID, "workspace of %lld bytes on 16: %lld needed", (long long)d->workspace_bytes, (long long)need);
-  PAGED_TRY(rows_launch(c, paged, d->dtype == QTB_T_F16, (int)d->head_dim, dev->sms, INT_MAX, d->workspace,
-                        static_cast<cudaStream_t>(stream)));
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool f16 = d->dtype == QTB_T_F16;
+  const int hd = (int)d->head_dim;
+  TileMaps maps;
+  const bool tiles = tile_maps(c, paged, f16, hd, dev->encode, maps);
+  const int limit = tiles ? ROWS_M : INT_MAX;
+  PAGED_TRY(rows_launch(c, paged, f16, hd, dev->sms, limit, d->workspace, st));
+  if (tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, maps, dev->sms, limit, st));
   return QTB_OK;
 }
 

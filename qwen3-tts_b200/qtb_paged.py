@@ -29,10 +29,10 @@ import torch
 
 import qtts_b200 as Q
 
-NO_PAGES, ROW_FULL, ROOM, LENGTH, PAGE = 1, 2, 4, 8, 16
+NO_PAGES, ROW_FULL, ROOM, LENGTH, PAGE, TIMEOUT = 1, 2, 4, 8, 16, 32
 _STATUS = {NO_PAGES: "the free list ran out", ROW_FULL: "a request outgrew its table row",
            ROOM: "more new tokens than max_tokens", LENGTH: "a negative length",
-           PAGE: "a page or slot outside the pool"}
+           PAGE: "a page or slot outside the pool", TIMEOUT: "a wait inside a kernel ran out"}
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 # the descriptors of include/qwen3tts_b200.h, field by field (all 64 bits wide)
