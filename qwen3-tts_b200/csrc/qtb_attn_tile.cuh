@@ -48,13 +48,18 @@ constexpr int tile_kv_bytes() { return TILE_N * HD * 2; }
 template <int HD>
 constexpr int tile_smem() { return 1024 + 2 * TILE_M * HD * 2 + tile_stages<HD>() * tile_kv_bytes<HD>(); }
 
+template <bool V>
+struct Flag {
+  static constexpr bool value = V;
+};
+
 struct TileMaps {
   CUtensorMap q, k, v;
 };
 
 struct TileSync {
   uint64_t q_full, q_empty, drain;
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
   uint64_t kv_full[8], kv_empty[8];
   uint32_t tmem;
   int abort;
@@ -116,10 +121,68 @@ QTB_DEV void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z,
       "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
       : "memory");
 }
+// Whether the phase has completed, after waiting a short while for it.
+QTB_DEV bool mbar_try(uint64_t *bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return done != 0;
+}
+// True in one lane of the (converged) warp, always the same one.
+QTB_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
 QTB_DEV float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// Two f32 values in a register pair, and their sum / product-sum in one instruction.
+QTB_DEV uint64_t f2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+QTB_DEV void f2_get(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+QTB_DEV uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+QTB_DEV uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two values <= 8 on the FMA pipe: 2^x = 2^n 2^f with n = x rounded (the
+// low bits of x + 1.5 * 2^23) and 2^f, |f| <= 1/2, by the polynomial of degree
+// 4 with the least largest relative error, 2.6e-6 (an exchange fit in 64 bits).
+// Below 2^-126 it gives that.
+QTB_DEV uint64_t exp2_poly2(uint64_t x) {
+  float a, b, ta, tb;
+  f2_get(x, a, b);
+  x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+  const uint64_t t = add2(x, f2(12582912.f, 12582912.f));
+  const uint64_t f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
+  uint64_t p = fma2(f, f2(0.009570102f, 0.009570102f), f2(0.055917859f, 0.055917859f));
+  p = fma2(p, f, f2(0.24024744f, 0.24024744f));
+  p = fma2(p, f, f2(0.69312179f, 0.69312179f));
+  p = fma2(p, f, f2(0.99999928f, 0.99999928f));
+  f2_get(p, a, b);
+  f2_get(t, ta, tb);
+  return f2(__int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23)));
 }
 
 // One unit of work: 2 tpt tokens (a tile pair) of a request, one key head.
@@ -137,12 +200,15 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int box) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
+  constexpr int P_FIRST = 3;               // 32-key quarters of P that are handed over first
+  constexpr int POLY = HD == 128 ? 4 : 2;  // of POLY exponentials one runs on the FMA pipe, not the MUFU
   extern __shared__ unsigned char smem_raw[];
   __shared__ TileSync sy;
   __shared__ int s_pre[TILE_SEGS + 1];
   unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char *s_q = smem, *s_kv = smem + 2 * Q_B;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // known to be the same in the whole warp
   const int tpt = TILE_M / c.group;        // tokens of a tile
 
   // --- pairs of every request (those with more than row_limit rows), summed
@@ -160,8 +226,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   if (tid == 0) {
     mbar_init(&sy.q_full, 1); mbar_init(&sy.q_empty, 1); mbar_init(&sy.drain, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i], 128);
-      mbar_init(&sy.o_full[i], 1); mbar_init(&sy.o_empty[i], 128);
+      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i][0], 4); mbar_init(&sy.p_full[i][1], 4);
+      mbar_init(&sy.o_full[i], 1); mbar_init(&sy.o_empty[i], 4);
     }
     for (int i = 0; i < STAGES; i++) { mbar_init(&sy.kv_full[i], 1); mbar_init(&sy.kv_empty[i], 1); }
     sy.abort = 0;
@@ -191,9 +257,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   const int pairs = s_pre[TILE_SEGS];
   const long long items = (long long)pairs * c.n_kv;
 
-  // Item i of the call, longest causal tiles first: pairs from the last to the
-  // first, key heads inside.  False past the end.
-  auto get_item = [&](long long i, TileItem &it) {
+  // This block's n-th item.  Items go longest causal tiles first (pairs from the
+  // last to the first, key heads inside) and are dealt to the blocks to and fro,
+  // so that the sums come out alike.  False past the end.
+  auto get_item = [&](int n, TileItem &it) {
+    const long long i = (long long)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     if (i >= items) return false;
     it.h = (int)(i % c.n_kv);
     int p = pairs - 1 - (int)(i / c.n_kv);
@@ -222,13 +290,16 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   };
   // Bounded wait of a whole warp; false: this or another role gave up.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    bool ok = mbar_wait(bar, parity, 20000);
-    const long long t0 = clock64();
-    while (!ok && !*reinterpret_cast<volatile int *>(&sy.abort)) {
-      ok = mbar_wait(bar, parity, 20000);
-      if (!ok && clock64() - t0 > TILE_WAIT) {
-        *reinterpret_cast<volatile int *>(&sy.abort) = 1;
-        raise_status(c.status, QTB_PS_TIMEOUT);
+    bool ok = mbar_try(bar, parity);
+    if (!ok) {
+      const long long t0 = clock64();
+      for (int n = 0; !(ok = mbar_try(bar, parity)); n++) {
+        if ((n & 15) != 15) continue;
+        if (*reinterpret_cast<volatile int *>(&sy.abort)) break;
+        if (clock64() - t0 > TILE_WAIT) {
+          *reinterpret_cast<volatile int *>(&sy.abort) = 1;
+          raise_status(c.status, QTB_PS_TIMEOUT);
+        }
       }
     }
     return (bool)__all_sync(0xffffffffu, ok);
@@ -241,7 +312,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     int bad = 0;
     uint32_t fill = 0, n_items = 0;        // ring fills issued; items begun
     bool ok = true;
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+    for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
       const int tiles = max(it.n[0], it.n[1]);
@@ -303,7 +374,10 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     const uint32_t idesc_s = umma_idesc(1u, ab, TILE_N), idesc_o = umma_idesc(1u, ab, HD) | (1u << 16);   // B as [K][N]
     uint32_t fill = 0, n_items = 0, p_n[2] = {0, 0}, o_n[2] = {0, 0};
     bool ok = true, issued = false;
-    for (long long i = blockIdx.x; ok; i += gridDim.x) {
+    // descriptors of the first tile and stage: others are an address (in 16 bytes) further on
+    const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_kv));
+    const uint64_t v_desc = umma_desc_mn128(smem_u32(s_kv), HALF_B);
+    for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
       const int tiles = max(it.n[0], it.n[1]);
@@ -311,12 +385,13 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       if (!wait(&sy.q_full, n_items & 1)) break;
       n_items++;
       auto scores = [&](int t, int st) {
-        if (lane == 0) {
-          const uint32_t q = smem_u32(s_q + t * Q_B), k = smem_u32(s_kv + st * KV_B);
+        const uint64_t q = q_desc + (uint32_t)(t * (Q_B >> 4)), k = k_desc + (uint32_t)(st * (KV_B >> 4));
+        const uint32_t d = tmem + S_COL + t * 128;
+        if (elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ks++) {
-            const uint32_t o = (ks >> 2) * HALF_B + (ks & 3) * 32;
-            umma_bf16(tmem + S_COL + t * 128, umma_desc_sw128(q + o), umma_desc_sw128(k + o), idesc_s, ks != 0);
+            const uint32_t o = ((ks >> 2) * HALF_B + (ks & 3) * 32) >> 4;
+            umma_bf16(d, q + o, k + o, idesc_s, ks != 0);
           }
           umma_commit(&sy.s_full[t]);
         }
@@ -327,10 +402,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       issued = true;
       for (int t = 0; t < 2; t++)
         if (it.n[t] > 0) scores(t, st);
-      if (lane == 0) {
+      if (elect_one()) {
         umma_commit(&sy.kv_empty[st]);
         if (tiles == 1) umma_commit(&sy.q_empty);
       }
+      __syncwarp();
       fill++;
       for (int j = 0; j < tiles && ok; j++) {
         const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
@@ -339,32 +415,37 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         for (int t = 0; t < 2 && ok; t++) {
           if (j >= it.n[t]) continue;
           if (j == 0 && !(ok = wait(&sy.o_empty[t], (o_n[t] & 1) ^ 1))) break;
-          if (!(ok = wait(&sy.p_full[t], p_n[t] & 1))) break;
-          p_n[t]++;
-          tc_fence_after();
-          if (lane == 0) {
-            const uint32_t v = smem_u32(s_kv + sv * KV_B);
 #pragma unroll
-            for (int ks = 0; ks < TILE_N / 16; ks++)
-              umma_ts(tmem + O_COL + t * HD, tmem + S_COL + t * 128 + ks * 8, umma_desc_mn128(v + ks * 2048, HALF_B), idesc_o,
-                      (j | ks) != 0);
-            if (j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
+          for (int part = 0; part < 2 && ok; part++) {   // the first keys' product starts while the last ones' P is made
+            if (!(ok = wait(&sy.p_full[t][part], p_n[t] & 1))) break;
+            tc_fence_after();
+            const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
+            const uint32_t d = tmem + O_COL + t * HD, a = tmem + S_COL + t * 128;
+            if (elect_one()) {
+#pragma unroll
+              for (int ks = part ? P_FIRST * 2 : 0; ks < (part ? TILE_N / 16 : P_FIRST * 2); ks++)
+                umma_ts(d, a + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
+              if (part && j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
+          if (!ok) break;
+          p_n[t]++;
           if (j == it.n[t] - 1) o_n[t]++;
           if (j + 1 < it.n[t]) scores(t, sk);
         }
         if (!ok) break;
-        if (lane == 0) {
+        if (elect_one()) {
           umma_commit(&sy.kv_empty[sv]);
           if (j + 1 < tiles) umma_commit(&sy.kv_empty[sk]);
           if (j + 2 == tiles) umma_commit(&sy.q_empty);
         }
+        __syncwarp();
         fill += j + 1 < tiles ? 2 : 1;
       }
     }
     if (issued) {                          // nothing reads shared or tensor memory any more
-      if (lane == 0) umma_commit(&sy.drain);
+      if (elect_one()) umma_commit(&sy.drain);
       __syncwarp();
       mbar_wait(&sy.drain, 0, TILE_WAIT);
     }
@@ -376,7 +457,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + S_COL + t * 128 + lanes, o_at = tmem + O_COL + t * HD + lanes;
     uint32_t fill = 0, s_n = 0, o_n = 0;
-    for (long long i = blockIdx.x;; i += gridDim.x) {
+    for (int i = 0;; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
       const int tiles = max(it.n[0], it.n[1]), n = it.n[t];
@@ -400,7 +481,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
 #pragma unroll
         for (int x = 0; x < 4; x++) tmem_ld32_async(s_at + 32 * x, s + 32 * x);
         tmem_ld_wait();
-        if (kb + TILE_N - 1 > all_last || kb < all_first) {
+        const bool masked = kb + TILE_N - 1 > all_last || kb < all_first;
+        if (masked) {
           const int a = first - kb, b = last - kb;
 #pragma unroll
           for (int x = 0; x < 128; x++) s[x] = x >= a && x <= b ? s[x] : -INFINITY;
@@ -432,24 +514,6 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int part = 0; part < 4; part++) {
-          // rounded to the tensors' type for the product with V, as large as
-          // the result's own rounding; the sum is of the unrounded ones
-          uint32_t p[16];
-#pragma unroll
-          for (int x = 0; x < 16; x++) {
-            const float a = exp2_approx(fmaf(s[32 * part + 2 * x], c.scale_log2, -base));
-            const float b = exp2_approx(fmaf(s[32 * part + 2 * x + 1], c.scale_log2, -base));
-            sum[x & 1] += a;
-            sum[2 + (x & 1)] += b;
-            p[x] = pack2<F16>(a, b);
-          }
-          tmem_st16(s_at + 16 * part, p);
-        }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         if (kb < low || kb + TILE_N > high) {
           // keys that no row sees: their V may be anything, and 0 * NaN is NaN
           const uint32_t f = fill + 2 * j + 1;
@@ -464,9 +528,44 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
           }
           fence_proxy_async_smem();
         }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&sy.p_full[t]);
+        const float base = m == -INFINITY ? 0.f : m;
+        const uint64_t scale2 = f2(c.scale_log2, c.scale_log2), base2 = f2(-base, -base);
+        auto probabilities = [&](auto poly) {
+#pragma unroll
+        for (int part = 0; part < 4; part++) {
+          // rounded to the tensors' type for the product with V, as large as
+          // the result's own rounding; the sum is of the unrounded ones
+          uint32_t p[16];
+#pragma unroll
+          for (int x = 0; x < 16; x++) {
+            float &a = s[32 * part + 2 * x], &b = s[32 * part + 2 * x + 1];
+            const uint64_t e = fma2(f2(a, b), scale2, base2);
+            if (decltype(poly)::value && x % POLY == POLY - 1) {
+              f2_get(exp2_poly2(e), a, b);
+            } else {
+              f2_get(e, a, b);
+              a = exp2_approx(a);
+              b = exp2_approx(b);
+            }
+            p[x] = pack2<F16>(a, b);
+          }
+          tmem_st16(s_at + 16 * part, p);
+          if (part == P_FIRST - 1 || part == 3) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sy.p_full[t][part == 3]);
+          }
+        }
+        };
+        if (masked) probabilities(Flag<false>());   // 2^-inf has to be 0 there
+        else probabilities(Flag<true>());
+        uint64_t sum[4] = {f2(s[0], s[1]), f2(s[2], s[3]), f2(s[4], s[5]), f2(s[6], s[7])};
+#pragma unroll
+        for (int x = 4; x < 64; x++) sum[x & 3] = add2(sum[x & 3], f2(s[2 * x], s[2 * x + 1]));
+        float la, lb;
+        f2_get(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), la, lb);
+        l += la + lb;
       }
       if (!ok) break;
       fill += 2 * tiles;
@@ -500,7 +599,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       }
       if (n > 0) {
         tc_fence_before();
-        mbar_arrive(&sy.o_empty[t]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sy.o_empty[t]);
       }
       if (live && c.lse) c.lse[tk * c.n_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
