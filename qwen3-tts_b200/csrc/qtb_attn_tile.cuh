@@ -59,7 +59,7 @@ struct TileMaps {
 
 struct TileSync {
   uint64_t q_full, q_empty, drain;
-  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
   uint64_t kv_full[8], kv_empty[8];
   uint32_t tmem;
   int abort;
@@ -200,8 +200,7 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int box) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
-  constexpr int P_FIRST = 3;               // 32-key quarters of P that are handed over first
-  constexpr int POLY = HD == 128 ? 4 : 2;  // of POLY exponentials one runs on the FMA pipe, not the MUFU
+  constexpr int POLY = 4;  // of POLY exponentials one runs on the FMA pipe, not the MUFU
   extern __shared__ unsigned char smem_raw[];
   __shared__ TileSync sy;
   __shared__ int s_pre[TILE_SEGS + 1];
@@ -226,7 +225,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   if (tid == 0) {
     mbar_init(&sy.q_full, 1); mbar_init(&sy.q_empty, 1); mbar_init(&sy.drain, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i][0], 4); mbar_init(&sy.p_full[i][1], 4);
+      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i], 4);
       mbar_init(&sy.o_full[i], 1); mbar_init(&sy.o_empty[i], 4);
     }
     for (int i = 0; i < STAGES; i++) { mbar_init(&sy.kv_full[i], 1); mbar_init(&sy.kv_empty[i], 1); }
@@ -410,38 +409,38 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       fill++;
       for (int j = 0; j < tiles && ok; j++) {
         const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
-        if (!(ok = wait(&sy.kv_full[sv], (fill / STAGES) & 1))) break;
-        if (j + 1 < tiles && !(ok = wait(&sy.kv_full[sk], ((fill + 1) / STAGES) & 1))) break;
-        for (int t = 0; t < 2 && ok; t++) {
+        const bool more = j + 1 < tiles;
+        for (int t = 0; t < 2; t++) {
           if (j >= it.n[t]) continue;
-          if (j == 0 && !(ok = wait(&sy.o_empty[t], (o_n[t] & 1) ^ 1))) break;
-#pragma unroll
-          for (int part = 0; part < 2 && ok; part++) {   // the first keys' product starts while the last ones' P is made
-            if (!(ok = wait(&sy.p_full[t][part], p_n[t] & 1))) break;
-            tc_fence_after();
-            const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
-            const uint32_t d = tmem + O_COL + t * HD, a = tmem + S_COL + t * 128;
-            if (elect_one()) {
-#pragma unroll
-              for (int ks = part ? P_FIRST * 2 : 0; ks < (part ? TILE_N / 16 : P_FIRST * 2); ks++)
-                umma_ts(d, a + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
-              if (part && j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
-            }
-            __syncwarp();
-          }
-          if (!ok) break;
+          // P of this tile, and with it V of this step and K of the next (lanes
+          // wait for one each: the waits' latencies would add up)
+          uint64_t *bar = &sy.p_full[t];
+          uint32_t par = p_n[t] & 1;
+          if (lane == 1) { bar = &sy.kv_full[sv]; par = (fill / STAGES) & 1; }
+          if (lane == 2 && more) { bar = &sy.kv_full[sk]; par = ((fill + 1) / STAGES) & 1; }
+          if (lane == 3 && j == 0) { bar = &sy.o_empty[t]; par = (o_n[t] & 1) ^ 1; }
+          if (!(ok = wait(bar, par))) break;
           p_n[t]++;
+          tc_fence_after();
+          const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
+          const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = 0; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
+            if (j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
+          }
+          __syncwarp();
           if (j == it.n[t] - 1) o_n[t]++;
           if (j + 1 < it.n[t]) scores(t, sk);
         }
         if (!ok) break;
         if (elect_one()) {
           umma_commit(&sy.kv_empty[sv]);
-          if (j + 1 < tiles) umma_commit(&sy.kv_empty[sk]);
+          if (more) umma_commit(&sy.kv_empty[sk]);
           if (j + 2 == tiles) umma_commit(&sy.q_empty);
         }
         __syncwarp();
-        fill += j + 1 < tiles ? 2 : 1;
+        fill += more ? 2 : 1;
       }
     }
     if (issued) {                          // nothing reads shared or tensor memory any more
@@ -550,13 +549,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
             p[x] = pack2<F16>(a, b);
           }
           tmem_st16(s_at + 16 * part, p);
-          if (part == P_FIRST - 1 || part == 3) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&sy.p_full[t][part == 3]);
-          }
         }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sy.p_full[t]);
         };
         if (masked) probabilities(Flag<false>());   // 2^-inf has to be 0 there
         else probabilities(Flag<true>());

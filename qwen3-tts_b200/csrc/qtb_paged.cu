@@ -329,8 +329,10 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   const int hd = (int)d->head_dim;
   TileMaps maps;
   const bool tiles = tile_maps(c, paged, f16, hd, dev->encode, maps);
-  const int limit = tiles ? ROWS_M : INT_MAX;
-  PAGED_TRY(rows_launch(c, paged, f16, hd, dev->sms, limit, d->workspace, st));
+  // Which kernel has a request: few rows over a long cache want the split key
+  // axis of the rows kernel, many rows the tiles; prompts have no long cache.
+  const int limit = !tiles ? INT_MAX : paged ? ROWS_M : 0;
+  if (limit) PAGED_TRY(rows_launch(c, paged, f16, hd, dev->sms, limit, d->workspace, st));
   if (tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, maps, dev->sms, limit, st));
   return QTB_OK;
 }
