@@ -22,6 +22,8 @@
 // 2^8 below the true one, so p <= 2^8 and the sum stays exact to f32 rounding;
 // only when a row outgrows that are its O and l scaled.  The final O / l does
 // not depend on m.
+// The probabilities of a tile start from the old maximum at once, beside the new
+// maximum's search, and are thrown away in the rare tile that outgrows it.
 //
 // Products are issued in order, so the commit that completes S of tile j also
 // says that P V of tile j - 1 is in O: the softmax warps may scale O then.
@@ -36,9 +38,9 @@ namespace qtb {
 constexpr int TILE_THREADS = 384, TILE_M = 128, TILE_N = 128;
 // Registers of a thread: the block starts with 168 for each of its 384 threads
 // (64512 in all); the softmax warps, a row of S each, take what the loading and
-// issuing warpgroup gives up: 256 * 200 + 128 * 96 = 63488.
-constexpr int TILE_REGS_SOFTMAX = 200, TILE_REGS_OTHER = 96;
-constexpr int TILE_SEGS = 256;             // entries of the in-block search over requests
+// issuing warpgroup gives up: 256 * 208 + 128 * 80 = 63488.
+constexpr int TILE_REGS_SOFTMAX = 208, TILE_REGS_OTHER = 80;
+constexpr int TILE_SEGS = 128;             // entries of the in-block search over requests
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
 template <int HD>
@@ -46,12 +48,7 @@ constexpr int tile_stages() { return HD == 128 ? 5 : 8; }
 template <int HD>
 constexpr int tile_kv_bytes() { return TILE_N * HD * 2; }
 template <int HD>
-constexpr int tile_smem() { return 1024 + 2 * TILE_M * HD * 2 + tile_stages<HD>() * tile_kv_bytes<HD>(); }
-
-template <bool V>
-struct Flag {
-  static constexpr bool value = V;
-};
+constexpr int tile_operands() { return 2 * TILE_M * HD * 2 + tile_stages<HD>() * tile_kv_bytes<HD>(); }
 
 struct TileMaps {
   CUtensorMap q, k, v;
@@ -59,11 +56,20 @@ struct TileMaps {
 
 struct TileSync {
   uint64_t q_full, q_empty, drain;
-  uint64_t s_full[2], p_full[2], o_full[2], o_empty[2];
+  uint64_t s_full[2], p_full[2][2], o_full[2], o_empty[2];
   uint64_t kv_full[8], kv_empty[8];
   uint32_t tmem;
   int abort;
 };
+
+// What lies in shared memory behind the operands (which start it, on 1024 bytes).
+struct TileShared {
+  TileSync sy;
+  int pre[TILE_SEGS + 1];                  // query tile pairs before each run of requests
+};
+template <int HD>
+constexpr int tile_smem() { return tile_operands<HD>() + (int)sizeof(TileShared); }
+static_assert(tile_smem<128>() <= 232448 && tile_smem<64>() <= 232448, "shared memory of a block");
 
 // D (+)= A B with A in tensor memory.
 QTB_DEV void umma_ts(uint32_t d, uint32_t a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -91,11 +97,10 @@ QTB_DEV void tmem_ld32_async(uint32_t taddr, float *r) {
         "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(taddr));
 }
-QTB_DEV void tmem_ld16_async(uint32_t taddr, float *r) {
+QTB_DEV void tmem_ld8_async(uint32_t taddr, float *r) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
-        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
       : "r"(taddr));
 }
 QTB_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -104,6 +109,12 @@ QTB_DEV void tmem_st16(uint32_t taddr, const uint32_t *r) {
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
       ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+QTB_DEV void tmem_st8(uint32_t taddr, const uint32_t *r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
       : "memory");
 }
 QTB_DEV void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
@@ -166,25 +177,6 @@ QTB_DEV uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of two values <= 8 on the FMA pipe: 2^x = 2^n 2^f with n = x rounded (the
-// low bits of x + 1.5 * 2^23) and 2^f, |f| <= 1/2, by the polynomial of degree
-// 4 with the least largest relative error, 2.6e-6 (an exchange fit in 64 bits).
-// Below 2^-126 it gives that.
-QTB_DEV uint64_t exp2_poly2(uint64_t x) {
-  float a, b, ta, tb;
-  f2_get(x, a, b);
-  x = f2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-  const uint64_t t = add2(x, f2(12582912.f, 12582912.f));
-  const uint64_t f = fma2(add2(t, f2(-12582912.f, -12582912.f)), f2(-1.f, -1.f), x);
-  uint64_t p = fma2(f, f2(0.009570102f, 0.009570102f), f2(0.055917859f, 0.055917859f));
-  p = fma2(p, f, f2(0.24024744f, 0.24024744f));
-  p = fma2(p, f, f2(0.69312179f, 0.69312179f));
-  p = fma2(p, f, f2(0.99999928f, 0.99999928f));
-  f2_get(p, a, b);
-  f2_get(t, ta, tb);
-  return f2(__int_as_float(__float_as_int(a) + (__float_as_int(ta) << 23)), __int_as_float(__float_as_int(b) + (__float_as_int(tb) << 23)));
-}
-
 // One unit of work: 2 tpt tokens (a tile pair) of a request, one key head.
 struct TileItem {
   AttnReq a;
@@ -200,11 +192,11 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int box) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
-  constexpr int POLY = 4;  // of POLY exponentials one runs on the FMA pipe, not the MUFU
-  extern __shared__ unsigned char smem_raw[];
-  __shared__ TileSync sy;
-  __shared__ int s_pre[TILE_SEGS + 1];
-  unsigned char *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+  constexpr int P_FIRST = 2;               // 32-key quarters of P that are handed over first
+  extern __shared__ __align__(1024) unsigned char smem[];
+  TileShared &sh = *reinterpret_cast<TileShared *>(smem + tile_operands<HD>());
+  TileSync &sy = sh.sy;
+  int *s_pre = sh.pre;
   unsigned char *s_q = smem, *s_kv = smem + 2 * Q_B;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // known to be the same in the whole warp
@@ -225,7 +217,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   if (tid == 0) {
     mbar_init(&sy.q_full, 1); mbar_init(&sy.q_empty, 1); mbar_init(&sy.drain, 1);
     for (int i = 0; i < 2; i++) {
-      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i], 4);
+      mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i][0], 4); mbar_init(&sy.p_full[i][1], 4);
       mbar_init(&sy.o_full[i], 1); mbar_init(&sy.o_empty[i], 4);
     }
     for (int i = 0; i < STAGES; i++) { mbar_init(&sy.kv_full[i], 1); mbar_init(&sy.kv_empty[i], 1); }
@@ -233,7 +225,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     fence_mbar_init();
   }
   __syncthreads();
-  if (warp == 0) {                         // exclusive sums: a lane has 32 entries
+  if (warp == 0) {                         // exclusive sums, a run of entries to a lane
     int v[TILE_SEGS / 32], sum = 0;
 #pragma unroll
     for (int i = 0; i < TILE_SEGS / 32; i++) { v[i] = s_pre[lane * (TILE_SEGS / 32) + i]; sum += v[i]; }
@@ -412,21 +404,28 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         const bool more = j + 1 < tiles;
         for (int t = 0; t < 2; t++) {
           if (j >= it.n[t]) continue;
-          // P of this tile, and with it V of this step and K of the next (lanes
-          // wait for one each: the waits' latencies would add up)
-          uint64_t *bar = &sy.p_full[t];
+          // The first part of P of this tile, and with it V of this step and K of the
+          // next (lanes wait for one each: the waits' latencies would add up).
+          uint64_t *bar = &sy.p_full[t][0];
           uint32_t par = p_n[t] & 1;
           if (lane == 1) { bar = &sy.kv_full[sv]; par = (fill / STAGES) & 1; }
           if (lane == 2 && more) { bar = &sy.kv_full[sk]; par = ((fill + 1) / STAGES) & 1; }
           if (lane == 3 && j == 0) { bar = &sy.o_empty[t]; par = (o_n[t] & 1) ^ 1; }
           if (!(ok = wait(bar, par))) break;
-          p_n[t]++;
           tc_fence_after();
           const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
           const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
+            for (int ks = 0; ks < P_FIRST * 2; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
+          }
+          __syncwarp();
+          if (!(ok = wait(&sy.p_full[t][1], p_n[t] & 1))) break;
+          p_n[t]++;
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int ks = P_FIRST * 2; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, 1);
             if (j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
           }
           __syncwarp();
@@ -460,108 +459,124 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       TileItem it;
       if (!get_item(i, it)) break;
       const int tiles = max(it.n[0], it.n[1]), n = it.n[t];
-      const int tt = row / c.group, tok = it.tok + t * tpt + tt, pos = it.a.first + tok;
-      const bool live = tt < it.n_tok[t];
-      const int last = min(c.causal ? pos : it.a.hi - 1, it.a.hi - 1);
-      const int first = c.window > 0 ? max(pos - c.window + 1, 0) : 0;
-      // what every row of the tile sees of a key tile lies within these
-      const int pos_a = it.a.first + it.tok + t * tpt, pos_b = pos_a + it.n_tok[t] - 1;
-      const int all_last = min(c.causal ? pos_a : it.a.hi - 1, it.a.hi - 1);
-      const int all_first = c.window > 0 ? max(pos_b - c.window + 1, 0) : 0;
+      const int tt = row / c.group;
+      const int pos = it.a.first + it.tok + t * tpt + tt;         // this row's position
+      const int tk = tt < it.n_tok[t] ? it.a.t0 + it.tok + t * tpt + tt : -1;   // its packed token (-1: no row)
+      const int head = it.h * c.group + row - tt * c.group;
       const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0, high = max(it.hi[0], it.hi[1]);
+      // key tiles [clear_a, clear_b) are seen whole by every row of the tile
+      const int pos_a = pos - tt, pos_b = pos_a + it.n_tok[t] - 1;
+      const int all_last = min(c.causal ? pos_a : it.a.hi - 1, it.a.hi - 1);
+      const int clear_a = c.window > 0 ? (max(pos_b - c.window + 1, 0) - it.k0 + TILE_N - 1) / TILE_N : 0;
+      const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
       for (int j = 0; j < n; j++) {
         if (!(ok = wait(&sy.s_full[t], s_n & 1))) break;
         s_n++;
         tc_fence_after();
-        const int kb = it.k0 + j * TILE_N;
         float s[128];
 #pragma unroll
         for (int x = 0; x < 4; x++) tmem_ld32_async(s_at + 32 * x, s + 32 * x);
         tmem_ld_wait();
-        const bool masked = kb + TILE_N - 1 > all_last || kb < all_first;
+        const bool masked = j < clear_a || j >= clear_b;
         if (masked) {
-          const int a = first - kb, b = last - kb;
+          const int kb = it.k0 + j * TILE_N;
+          const int a = (c.window > 0 ? max(pos - c.window + 1, 0) : 0) - kb, b = min(c.causal ? pos : it.a.hi - 1, it.a.hi - 1) - kb;
 #pragma unroll
           for (int x = 0; x < 128; x++) s[x] = x >= a && x <= b ? s[x] : -INFINITY;
-        }
-        float mx[4];
+          if (kb < low || kb + TILE_N > high) {
+            // keys that no row sees: their V may be anything, and 0 * NaN is NaN
+            const uint32_t f = fill + 2 * j + 1;
+            unsigned char *v = s_kv + (f % STAGES) * KV_B;
+            if (!(ok = wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1))) break;
+            if (kb + row < low || kb + row >= high) {
 #pragma unroll
-        for (int x = 0; x < 4; x++) mx[x] = max3(s[x], s[x + 4], s[x + 8]);
+              for (int x = 0; x < HD / 64; x++)
 #pragma unroll
-        for (int x = 12; x + 8 <= 128; x += 8)
-#pragma unroll
-          for (int y = 0; y < 4; y++) mx[y] = max3(mx[y], s[x + y], s[x + 4 + y]);
-#pragma unroll
-        for (int y = 0; y < 4; y++) mx[y] = fmaxf(mx[y], s[124 + y]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c.scale_log2;
-        if (__any_sync(0xffffffffu, top > m + 8.f)) {
-          const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_approx(m - m2);
-          m = m2;
-          l *= f;
-          if (j > 0) {
-#pragma unroll 1
-            for (int x = 0; x < HD / 16; x++) {
-              float o[16];
-              uint32_t w[16];
-              tmem_ld16_async(o_at + 16 * x, o);
-              tmem_ld_wait();
-#pragma unroll
-              for (int y = 0; y < 16; y++) w[y] = __float_as_uint(o[y] * f);
-              tmem_st16(o_at + 16 * x, w);
+                for (int y = 0; y < 8; y++)
+                  *reinterpret_cast<uint4 *>(v + x * HALF_B + row * 128 + y * 16) = make_uint4(0, 0, 0, 0);
             }
+            fence_proxy_async_smem();
           }
         }
-        if (kb < low || kb + TILE_N > high) {
-          // keys that no row sees: their V may be anything, and 0 * NaN is NaN
-          const uint32_t f = fill + 2 * j + 1;
-          unsigned char *v = s_kv + (f % STAGES) * KV_B;
-          if (!(ok = wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1))) break;
-          if (kb + row < low || kb + row >= high) {
+        auto maximum = [&]() {
+          float mx[4];
 #pragma unroll
-            for (int x = 0; x < HD / 64; x++)
+          for (int x = 0; x < 4; x++) mx[x] = max3(s[x], s[x + 4], s[x + 8]);
 #pragma unroll
-              for (int y = 0; y < 8; y++)
-                *reinterpret_cast<uint4 *>(v + x * HALF_B + row * 128 + y * 16) = make_uint4(0, 0, 0, 0);
-          }
-          fence_proxy_async_smem();
-        }
-        const float base = m == -INFINITY ? 0.f : m;
-        const uint64_t scale2 = f2(c.scale_log2, c.scale_log2), base2 = f2(-base, -base);
-        auto probabilities = [&](auto poly) {
+          for (int x = 12; x + 8 <= 128; x += 8)
 #pragma unroll
-        for (int part = 0; part < 4; part++) {
-          // rounded to the tensors' type for the product with V, as large as
-          // the result's own rounding; the sum is of the unrounded ones
+            for (int y = 0; y < 4; y++) mx[y] = max3(mx[y], s[x + y], s[x + 4 + y]);
+#pragma unroll
+          for (int y = 0; y < 4; y++) mx[y] = fmaxf(mx[y], s[124 + y]);
+          return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * c.scale_log2;
+        };
+        const uint64_t scale2 = f2(c.scale_log2, c.scale_log2);
+        uint64_t sum[2];
+        // Probabilities of keys 32 part .. 32 part + 31 to tensor memory, rounded to
+        // the tensors' type for the product with V, as large as the result's own
+        // rounding; the sum is of the unrounded ones.
+        auto probabilities = [&](int part) {
+          const float base = m == -INFINITY ? 0.f : m;
+          const uint64_t base2 = f2(-base, -base);
           uint32_t p[16];
 #pragma unroll
           for (int x = 0; x < 16; x++) {
-            float &a = s[32 * part + 2 * x], &b = s[32 * part + 2 * x + 1];
-            const uint64_t e = fma2(f2(a, b), scale2, base2);
-            if (decltype(poly)::value && x % POLY == POLY - 1) {
-              f2_get(exp2_poly2(e), a, b);
-            } else {
-              f2_get(e, a, b);
-              a = exp2_approx(a);
-              b = exp2_approx(b);
-            }
+            float a, b;
+            f2_get(fma2(f2(s[32 * part + 2 * x], s[32 * part + 2 * x + 1]), scale2, base2), a, b);
+            a = exp2_approx(a);
+            b = exp2_approx(b);
+            sum[x & 1] = add2(sum[x & 1], f2(a, b));
             p[x] = pack2<F16>(a, b);
           }
           tmem_st16(s_at + 16 * part, p);
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sy.p_full[t]);
         };
-        if (masked) probabilities(Flag<false>());   // 2^-inf has to be 0 there
-        else probabilities(Flag<true>());
-        uint64_t sum[4] = {f2(s[0], s[1]), f2(s[2], s[3]), f2(s[4], s[5]), f2(s[6], s[7])};
+        auto hand_over = [&](int part) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sy.p_full[t][part]);
+        };
+        // Past the first tile m rarely moves: the probabilities start from the old
+        // one while the maximum is taken beside them, and are made anew where a row
+        // has outgrown it.
+        bool anew = j == 0;
+        if (!anew) {
+          sum[0] = sum[1] = 0;
 #pragma unroll
-        for (int x = 4; x < 64; x++) sum[x & 3] = add2(sum[x & 3], f2(s[2 * x], s[2 * x + 1]));
+          for (int part = 0; part < P_FIRST; part++) probabilities(part);
+          anew = __any_sync(0xffffffffu, maximum() > m + 8.f);
+        }
+        if (anew) {
+          const float top = maximum();
+          if (__any_sync(0xffffffffu, top > m + 8.f)) {
+            const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_approx(m - m2);
+            m = m2;
+            l *= f;
+            if (j > 0) {
+#pragma unroll 1
+              for (int x = 0; x < HD / 8; x++) {
+                float o[8];
+                uint32_t w[8];
+                tmem_ld8_async(o_at + 8 * x, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int y = 0; y < 8; y++) w[y] = __float_as_uint(o[y] * f);
+                tmem_st8(o_at + 8 * x, w);
+              }
+            }
+          }
+          sum[0] = sum[1] = 0;
+#pragma unroll
+          for (int part = 0; part < P_FIRST; part++) probabilities(part);
+        }
+        hand_over(0);
+#pragma unroll
+        for (int part = P_FIRST; part < 4; part++) probabilities(part);
+        hand_over(1);
         float la, lb;
-        f2_get(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), la, lb);
+        f2_get(add2(sum[0], sum[1]), la, lb);
         l += la + lb;
       }
       if (!ok) break;
@@ -571,10 +586,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         o_n++;
         tc_fence_after();
       }
-      const long long tk = it.a.t0 + tok;
-      const int h = it.h * c.group + row - tt * c.group;
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
-      uint16_t *op = c.out + tk * c.o_st + h * c.o_sh;
+      uint16_t *op = c.out + (long long)tk * c.o_st + head * c.o_sh;
 #pragma unroll
       for (int x = 0; x < HD / 32; x++) {
         float o[32];
@@ -582,7 +595,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
           tmem_ld32_async(o_at + 32 * x, o);
           tmem_ld_wait();
         }
-        if (live) {
+        if (tk >= 0) {
 #pragma unroll
           for (int y = 0; y < 4; y++) {
             uint32_t w[4];
@@ -599,7 +612,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         __syncwarp();
         if (lane == 0) mbar_arrive(&sy.o_empty[t]);
       }
-      if (live && c.lse) c.lse[tk * c.n_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      if (tk >= 0 && c.lse) c.lse[(long long)tk * c.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
   }
   tc_fence_before();
