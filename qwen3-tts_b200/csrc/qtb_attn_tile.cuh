@@ -38,9 +38,9 @@ namespace qtb {
 constexpr int TILE_THREADS = 384, TILE_M = 128, TILE_N = 128;
 // Registers of a thread: the block starts with 168 for each of its 384 threads
 // (64512 in all); the softmax warps, a row of S each, take what the loading and
-// issuing warpgroup gives up: 256 * 208 + 128 * 80 = 63488.
-constexpr int TILE_REGS_SOFTMAX = 208, TILE_REGS_OTHER = 80;
-constexpr int TILE_SEGS = 128;             // entries of the in-block search over requests
+// issuing warpgroup gives up: 256 * 200 + 128 * 96 = 63488.
+constexpr int TILE_REGS_SOFTMAX = 200, TILE_REGS_OTHER = 96;
+constexpr int TILE_SEGS = 128;             // runs of requests that the in-block search tells apart
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
 template <int HD>
@@ -66,6 +66,7 @@ struct TileSync {
 struct TileShared {
   TileSync sy;
   int pre[TILE_SEGS + 1];                  // query tile pairs before each run of requests
+  int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS];   // the requests themselves, where a run is one
 };
 template <int HD>
 constexpr int tile_smem() { return tile_operands<HD>() + (int)sizeof(TileShared); }
@@ -179,20 +180,20 @@ QTB_DEV uint64_t add2(uint64_t a, uint64_t b) {
 }
 // One unit of work: 2 tpt tokens (a tile pair) of a request, one key head.
 struct TileItem {
-  AttnReq a;
-  int r, h, tok;        // request, key head, first token of the pair
-  int n_tok[2];         // tokens in each tile
+  int r, h, t0, tok;    // request, key head, the request's first packed token, first token of the pair
+  int first, end;       // position of the request's token 0, its keys
+  int low;              // keys before this are seen by no row of the pair
   int k0;               // first key of key tile 0 (a multiple of 128)
-  int n[2];             // key tiles of each query tile
-  int hi[2];            // keys at and past this are seen by no row of the tile
+  int tok0, tok1;       // tokens in each tile
+  int n0, n1;           // key tiles of each
+  int high;             // keys at and past this are seen by no row
 };
 
 template <int HD, bool F16, bool PAGED>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
-tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int box) {
+tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int tpt, int box) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
-  constexpr int P_FIRST = 2;               // 32-key quarters of P that are handed over first
   extern __shared__ __align__(1024) unsigned char smem[];
   TileShared &sh = *reinterpret_cast<TileShared *>(smem + tile_operands<HD>());
   TileSync &sy = sh.sy;
@@ -200,21 +201,14 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   unsigned char *s_q = smem, *s_kv = smem + 2 * Q_B;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // known to be the same in the whole warp
-  const int tpt = TILE_M / c.group;        // tokens of a tile
-
-  // --- pairs of every request (those with more than row_limit rows), summed
-  const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS, n_seg = (c.n_req + seg - 1) / seg;
-  auto pairs_of = [&](int r) {
-    const int n = attn_request<PAGED>(c, r).n;
-    return n * c.group > row_limit ? (n + 2 * tpt - 1) / (2 * tpt) : 0;
-  };
-  for (int s = tid; s < TILE_SEGS; s += TILE_THREADS) {
-    int sum = 0;
-    if (s < n_seg)
-      for (int r = s * seg; r < min((s + 1) * seg, c.n_req); r++) sum += pairs_of(r);
-    s_pre[s] = sum;
-  }
-  if (tid == 0) {
+  if (warp == 8) {
+    if (lane < 3) {
+      const CUtensorMap *m = lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v;
+      asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+    }
+  } else if (warp == 9) {
+    tmem_alloc(&sy.tmem, 512);
+  } else if (tid == 10 * 32) {
     mbar_init(&sy.q_full, 1); mbar_init(&sy.q_empty, 1); mbar_init(&sy.drain, 1);
     for (int i = 0; i < 2; i++) {
       mbar_init(&sy.s_full[i], 1); mbar_init(&sy.p_full[i][0], 4); mbar_init(&sy.p_full[i][1], 4);
@@ -224,59 +218,77 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     sy.abort = 0;
     fence_mbar_init();
   }
-  __syncthreads();
-  if (warp == 0) {                         // exclusive sums, a run of entries to a lane
-    int v[TILE_SEGS / 32], sum = 0;
-#pragma unroll
-    for (int i = 0; i < TILE_SEGS / 32; i++) { v[i] = s_pre[lane * (TILE_SEGS / 32) + i]; sum += v[i]; }
-    int pre = sum;
+  // --- pairs of every request (those with more than row_limit rows), summed over
+  // runs of requests: one of the first 128 threads has a run
+  const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS;
+  auto pairs_of = [&](int n) { return n * c.group > row_limit ? (n + 2 * tpt - 1) / (2 * tpt) : 0; };
+  int sum = 0, pre = 0;
+  if (tid < TILE_SEGS) {
+    for (int r = tid * seg; r < min((tid + 1) * seg, c.n_req); r++) {
+      const AttnReq a = attn_request<PAGED>(c, r);
+      sum += pairs_of(a.n);
+      sh.t0[tid] = a.t0; sh.n[tid] = a.n; sh.hi[tid] = a.hi;
+    }
+    pre = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int x = __shfl_up_sync(0xffffffffu, pre, o);
       if (lane >= o) pre += x;
     }
-    if (lane == 31) s_pre[TILE_SEGS] = pre;
-    pre -= sum;
-#pragma unroll
-    for (int i = 0; i < TILE_SEGS / 32; i++) { s_pre[lane * (TILE_SEGS / 32) + i] = pre; pre += v[i]; }
+    if (lane == 31) sh.pre[warp] = pre;
   }
-  if (warp == 1) tmem_alloc(&sy.tmem, 512);
+  __syncthreads();
+  int before = 0, pairs = 0;
+#pragma unroll
+  for (int w = 0; w < TILE_SEGS / 32; w++) {
+    const int x = sh.pre[w];
+    if (w < warp) before += x;
+    pairs += x;
+  }
+  __syncthreads();
+  if (tid < TILE_SEGS) sh.pre[tid] = before + pre - sum;
+  if (tid == 0) sh.pre[TILE_SEGS] = pairs;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sy.tmem;
-  const int pairs = s_pre[TILE_SEGS];
-  const long long items = (long long)pairs * c.n_kv;
+  const int items = pairs * c.n_kv;        // the host has bounded it
 
   // This block's n-th item.  Items go longest causal tiles first (pairs from the
   // last to the first, key heads inside) and are dealt to the blocks to and fro,
   // so that the sums come out alike.  False past the end.
   auto get_item = [&](int n, TileItem &it) {
-    const long long i = (long long)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (i >= items) return false;
-    it.h = (int)(i % c.n_kv);
-    int p = pairs - 1 - (int)(i / c.n_kv);
-    int lo = 0, hi = n_seg;                // s_pre[lo] <= p < s_pre[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s_pre[mid] <= p) lo = mid; else hi = mid;
+    const unsigned i = (unsigned)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if (i >= (unsigned)items) return false;
+    int p = (int)(i / (unsigned)c.n_kv);
+    it.h = (int)i - p * c.n_kv;
+    p = pairs - 1 - p;
+    int lo = 0;                            // the last run that starts at or before p
+#pragma unroll 1
+    for (int step = TILE_SEGS / 2; step; step >>= 1)
+      if (sh.pre[lo + step] <= p) lo += step;
+    p -= sh.pre[lo];
+    it.r = lo;
+    int n_tok = sh.n[lo];
+    it.t0 = sh.t0[lo];
+    it.end = sh.hi[lo];
+    if (seg > 1) {
+      it.r = lo * seg;
+      AttnReq a = attn_request<PAGED>(c, it.r);
+      for (int q; p >= (q = pairs_of(a.n)); a = attn_request<PAGED>(c, ++it.r)) p -= q;
+      n_tok = a.n; it.t0 = a.t0; it.end = a.hi;
     }
-    p -= s_pre[lo];
-    it.r = lo * seg;
-    for (int q; p >= (q = pairs_of(it.r)); it.r++) p -= q;
-    it.a = attn_request<PAGED>(c, it.r);
+    it.first = it.end - n_tok;
     it.tok = p * 2 * tpt;
-    const int left = it.a.n - it.tok;
-    it.n_tok[0] = min(left, tpt);
-    it.n_tok[1] = max(min(left - tpt, tpt), 0);
-    const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0;
-    it.k0 = low / TILE_N * TILE_N;
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-      const int end = it.a.first + it.tok + t * tpt + it.n_tok[t];   // one past the tile's last token
-      it.hi[t] = c.causal ? min(end, it.a.hi) : it.a.hi;
-      it.n[t] = it.n_tok[t] > 0 && it.hi[t] > low ? (it.hi[t] - it.k0 + TILE_N - 1) / TILE_N : 0;
-    }
+    it.tok0 = min(n_tok - it.tok, tpt);
+    it.tok1 = max(min(n_tok - it.tok - tpt, tpt), 0);
+    it.low = c.window > 0 ? max(it.first + it.tok - c.window + 1, 0) : 0;
+    it.k0 = it.low / TILE_N * TILE_N;
+    const int mid = it.first + it.tok + it.tok0;          // position past the tile's last token
+    const int hi0 = c.causal ? min(mid, it.end) : it.end, hi1 = c.causal ? min(mid + it.tok1, it.end) : it.end;
+    it.n0 = hi0 > it.low ? (hi0 - it.k0 + TILE_N - 1) / TILE_N : 0;
+    it.n1 = it.tok1 > 0 && hi1 > it.low ? (hi1 - it.k0 + TILE_N - 1) / TILE_N : 0;
+    it.high = max(hi0, hi1);
     return true;
   };
   // Bounded wait of a whole warp; false: this or another role gave up.
@@ -306,18 +318,16 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int tiles = max(it.n[0], it.n[1]);
+      const int tiles = max(it.n0, it.n1);
       if (tiles == 0) continue;
-      const int hi = max(it.hi[0], it.hi[1]);
-      const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0;
       auto load_q = [&]() {
         if (!wait(&sy.q_empty, (n_items & 1) ^ 1)) return false;
         if (lane == 0) {
-          const int rows = tpt * c.group, two = it.n_tok[1] > 0;
+          const int rows = tpt * c.group, two = it.tok1 > 0;
           mbar_arrive_expect_tx(&sy.q_full, (uint32_t)(rows * 128 * (HD / 64) * (1 + two)));
           for (int t = 0; t <= two; t++)
             for (int x = 0; x < HD / 64; x++)
-              tma_load_4d(s_q + t * Q_B + x * HALF_B, &maps.q, x * 64, it.h * c.group, it.a.t0 + it.tok + t * tpt, 0, &sy.q_full);
+              tma_load_4d(s_q + t * Q_B + x * HALF_B, &maps.q, x * 64, it.h * c.group, it.t0 + it.tok + t * tpt, 0, &sy.q_full);
         }
         n_items++;
         return true;
@@ -327,7 +337,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         // this lane's box of the key tile: positions [pos, pos + box), 64 dims
         const int boxes = PAGED ? TILE_N / box : 1, bi = lane / (HD / 64), x = lane % (HD / 64);
         const int pos = kb + bi * box;
-        const bool mine = bi < boxes && pos < hi && pos + box > low;
+        const bool mine = bi < boxes && pos < it.high && pos + box > it.low;
         int pg = 0, off = 0;
         if (PAGED && mine) {
           const int e = pos / c.page;
@@ -346,7 +356,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
             unsigned char *dst = s_kv + st * KV_B + x * HALF_B + bi * box * 128;
             const CUtensorMap *map = kv ? &maps.v : &maps.k;
             if (PAGED) tma_load_4d(dst, map, x * 64, off, it.h, pg, &sy.kv_full[st]);
-            else tma_load_4d(dst, map, x * 64, it.a.t0 + pos, it.h, 0, &sy.kv_full[st]);
+            else tma_load_4d(dst, map, x * 64, it.t0 + pos, it.h, 0, &sy.kv_full[st]);
           }
           fill++;
           // the queries' buffer may still serve the item before: its keys go first
@@ -363,7 +373,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     // --------------------------------------------------------------- MMA ---
     const uint32_t ab = F16 ? 0u : 1u;
     const uint32_t idesc_s = umma_idesc(1u, ab, TILE_N), idesc_o = umma_idesc(1u, ab, HD) | (1u << 16);   // B as [K][N]
-    uint32_t fill = 0, n_items = 0, p_n[2] = {0, 0}, o_n[2] = {0, 0};
+    uint32_t fill = 0, n_items = 0;
+    uint32_t p_n = 0, o_n = 0;             // bit t: parity of the P hand-overs, of the finished outputs of tile t
     bool ok = true, issued = false;
     // descriptors of the first tile and stage: others are an address (in 16 bytes) further on
     const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_kv));
@@ -371,7 +382,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int tiles = max(it.n[0], it.n[1]);
+      const int tiles = max(it.n0, it.n1);
       if (tiles == 0) continue;
       if (!wait(&sy.q_full, n_items & 1)) break;
       n_items++;
@@ -391,8 +402,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       int st = (int)(fill % STAGES);
       if (!(ok = wait(&sy.kv_full[st], (fill / STAGES) & 1))) break;
       issued = true;
-      for (int t = 0; t < 2; t++)
-        if (it.n[t] > 0) scores(t, st);
+      if (it.n0 > 0) scores(0, st);
+      if (it.n1 > 0) scores(1, st);
       if (elect_one()) {
         umma_commit(&sy.kv_empty[st]);
         if (tiles == 1) umma_commit(&sy.q_empty);
@@ -402,35 +413,37 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       for (int j = 0; j < tiles && ok; j++) {
         const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
         const bool more = j + 1 < tiles;
+#pragma unroll
         for (int t = 0; t < 2; t++) {
-          if (j >= it.n[t]) continue;
-          // The first part of P of this tile, and with it V of this step and K of the
+          const int n = t ? it.n1 : it.n0;
+          if (j >= n) continue;
+          // The first half of P of this tile, and with it V of this step and K of the
           // next (lanes wait for one each: the waits' latencies would add up).
           uint64_t *bar = &sy.p_full[t][0];
-          uint32_t par = p_n[t] & 1;
+          uint32_t par = (p_n >> t) & 1;
           if (lane == 1) { bar = &sy.kv_full[sv]; par = (fill / STAGES) & 1; }
           if (lane == 2 && more) { bar = &sy.kv_full[sk]; par = ((fill + 1) / STAGES) & 1; }
-          if (lane == 3 && j == 0) { bar = &sy.o_empty[t]; par = (o_n[t] & 1) ^ 1; }
+          if (lane == 3 && j == 0) { bar = &sy.o_empty[t]; par = ((o_n >> t) & 1) ^ 1; }
           if (!(ok = wait(bar, par))) break;
           tc_fence_after();
           const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
           const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < P_FIRST * 2; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
+            for (int ks = 0; ks < TILE_N / 32; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
           }
           __syncwarp();
-          if (!(ok = wait(&sy.p_full[t][1], p_n[t] & 1))) break;
-          p_n[t]++;
+          if (!(ok = wait(&sy.p_full[t][1], (p_n >> t) & 1))) break;
+          p_n ^= 1u << t;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
-            for (int ks = P_FIRST * 2; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, 1);
-            if (j == it.n[t] - 1) umma_commit(&sy.o_full[t]);
+            for (int ks = TILE_N / 32; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, 1);
+            if (j == n - 1) umma_commit(&sy.o_full[t]);
           }
           __syncwarp();
-          if (j == it.n[t] - 1) o_n[t]++;
-          if (j + 1 < it.n[t]) scores(t, sk);
+          if (j == n - 1) o_n ^= 1u << t;
+          if (j + 1 < n) scores(t, sk);
         }
         if (!ok) break;
         if (elect_one()) {
@@ -458,15 +471,14 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int i = 0;; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int tiles = max(it.n[0], it.n[1]), n = it.n[t];
+      const int tiles = max(it.n0, it.n1), n = t ? it.n1 : it.n0, n_tok = t ? it.tok1 : it.tok0;
       const int tt = row / c.group;
-      const int pos = it.a.first + it.tok + t * tpt + tt;         // this row's position
-      const int tk = tt < it.n_tok[t] ? it.a.t0 + it.tok + t * tpt + tt : -1;   // its packed token (-1: no row)
+      const int pos = it.first + it.tok + t * tpt + tt;           // this row's position
+      const int tk = tt < n_tok ? it.t0 + it.tok + t * tpt + tt : -1;   // its packed token (-1: no row)
       const int head = it.h * c.group + row - tt * c.group;
-      const int low = c.window > 0 ? max(it.a.first + it.tok - c.window + 1, 0) : 0, high = max(it.hi[0], it.hi[1]);
       // key tiles [clear_a, clear_b) are seen whole by every row of the tile
-      const int pos_a = pos - tt, pos_b = pos_a + it.n_tok[t] - 1;
-      const int all_last = min(c.causal ? pos_a : it.a.hi - 1, it.a.hi - 1);
+      const int pos_a = pos - tt, pos_b = pos_a + n_tok - 1;
+      const int all_last = min(c.causal ? pos_a : it.end - 1, it.end - 1);
       const int clear_a = c.window > 0 ? (max(pos_b - c.window + 1, 0) - it.k0 + TILE_N - 1) / TILE_N : 0;
       const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
       float m = -INFINITY, l = 0.f;
@@ -482,20 +494,25 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         const bool masked = j < clear_a || j >= clear_b;
         if (masked) {
           const int kb = it.k0 + j * TILE_N;
-          const int a = (c.window > 0 ? max(pos - c.window + 1, 0) : 0) - kb, b = min(c.causal ? pos : it.a.hi - 1, it.a.hi - 1) - kb;
+          // this row sees keys a .. b of the tile
+          const int a = max((c.window > 0 ? max(pos - c.window + 1, 0) : 0) - kb, 0);
+          const int b = min(c.causal ? pos : it.end - 1, it.end - 1) - kb;
 #pragma unroll
-          for (int x = 0; x < 128; x++) s[x] = x >= a && x <= b ? s[x] : -INFINITY;
-          if (kb < low || kb + TILE_N > high) {
+          for (int y = 0; y < 4; y++) {
+            const int u = min(max(a - 32 * y, 0), 32), w = min(max(b + 1 - 32 * y, 0), 32);   // keys u .. w - 1 of 32
+            const uint32_t seen = (uint32_t)((1ull << w) - 1) & ~(uint32_t)((1ull << u) - 1);
+#pragma unroll
+            for (int x = 0; x < 32; x++) s[32 * y + x] = seen & (1u << x) ? s[32 * y + x] : -INFINITY;
+          }
+          if (kb < it.low || kb + TILE_N > it.high) {
             // keys that no row sees: their V may be anything, and 0 * NaN is NaN
             const uint32_t f = fill + 2 * j + 1;
             unsigned char *v = s_kv + (f % STAGES) * KV_B;
             if (!(ok = wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1))) break;
-            if (kb + row < low || kb + row >= high) {
-#pragma unroll
-              for (int x = 0; x < HD / 64; x++)
-#pragma unroll
-                for (int y = 0; y < 8; y++)
-                  *reinterpret_cast<uint4 *>(v + x * HALF_B + row * 128 + y * 16) = make_uint4(0, 0, 0, 0);
+            if (kb + row < it.low || kb + row >= it.high) {
+#pragma unroll 1
+              for (int y = 0; y < 8 * (HD / 64); y++)
+                *reinterpret_cast<uint4 *>(v + (y >> 3) * HALF_B + row * 128 + (y & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();
           }
@@ -545,7 +562,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         if (!anew) {
           sum[0] = sum[1] = 0;
 #pragma unroll
-          for (int part = 0; part < P_FIRST; part++) probabilities(part);
+          for (int part = 0; part < 2; part++) probabilities(part);
           anew = __any_sync(0xffffffffu, maximum() > m + 8.f);
         }
         if (anew) {
@@ -569,11 +586,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
           }
           sum[0] = sum[1] = 0;
 #pragma unroll
-          for (int part = 0; part < P_FIRST; part++) probabilities(part);
+          for (int part = 0; part < 2; part++) probabilities(part);
         }
         hand_over(0);
 #pragma unroll
-        for (int part = P_FIRST; part < 4; part++) probabilities(part);
+        for (int part = 2; part < 4; part++) probabilities(part);
         hand_over(1);
         float la, lb;
         f2_get(add2(sum[0], sum[1]), la, lb);
@@ -587,24 +604,42 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         tc_fence_after();
       }
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
-      uint16_t *op = c.out + (long long)tk * c.o_st + head * c.o_sh;
+      // A thread has a row, so that its 16-byte stores would each touch a line of
+      // their own: four neighbours turn their 4 x 4 units first, and a store
+      // instruction writes 64 bytes of each of 8 rows.
+      const long long at = tk >= 0 ? (long long)tk * c.o_st + head * c.o_sh : -1;
+      long long rows[4];
 #pragma unroll
+      for (int y = 0; y < 4; y++) rows[y] = __shfl_sync(0xffffffffu, at, (lane & ~3) + y);
+#pragma unroll 1
       for (int x = 0; x < HD / 32; x++) {
         float o[32];
         if (n > 0) {
           tmem_ld32_async(o_at + 32 * x, o);
           tmem_ld_wait();
         }
-        if (tk >= 0) {
+        uint32_t w[4][4];
+#pragma unroll
+        for (int y = 0; y < 4; y++)
+#pragma unroll
+          for (int z = 0; z < 4; z++)
+            w[y][z] = n > 0 ? pack2<F16>(o[8 * y + 2 * z] * inv, o[8 * y + 2 * z + 1] * inv) : 0u;
+#pragma unroll
+        for (int bit = 1; bit <= 2; bit <<= 1)
 #pragma unroll
           for (int y = 0; y < 4; y++) {
-            uint32_t w[4];
+            if (y & bit) continue;
 #pragma unroll
-            for (int z = 0; z < 4; z++)
-              w[z] = n > 0 ? pack2<F16>(o[8 * y + 2 * z] * inv, o[8 * y + 2 * z + 1] * inv) : 0u;
-            *reinterpret_cast<uint4 *>(op + 32 * x + 8 * y) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int z = 0; z < 4; z++) {
+              const uint32_t got = __shfl_xor_sync(0xffffffffu, lane & bit ? w[y][z] : w[y | bit][z], bit);
+              if (lane & bit) w[y][z] = got;
+              else w[y | bit][z] = got;
+            }
           }
-        }
+#pragma unroll
+        for (int y = 0; y < 4; y++)
+          if (rows[y] >= 0)
+            *reinterpret_cast<uint4 *>(c.out + rows[y] + 32 * x + 8 * (lane & 3)) = make_uint4(w[y][0], w[y][1], w[y][2], w[y][3]);
         __syncwarp();
       }
       if (n > 0) {
@@ -618,7 +653,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 512);
+  if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
 // ------------------------------------------------------------------ host ---
@@ -669,7 +704,7 @@ template <int HD, bool F16, bool PAGED>
 static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, int grid, int row_limit, cudaStream_t st) {
   if (prepare)
     return cudaFuncSetAttribute(tile_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<HD>());
-  tile_kernel<HD, F16, PAGED><<<grid, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tile_box(PAGED, c->page));
+  tile_kernel<HD, F16, PAGED><<<grid, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, TILE_M / c->group, tile_box(PAGED, c->page));
   return cudaGetLastError();
 }
 static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int grid, int row_limit,

@@ -281,6 +281,8 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
   if (d->n_heads / d->n_kv > 128) return qtb_fail(QTB_E_UNSUPPORTED, "%lld query heads to a key head: at most 128", (long long)(d->n_heads / d->n_kv));
   if (d->n_req < 0 || d->n_req >= (1 << 24) || d->n_tokens < 0 || d->n_tokens * (d->n_heads / d->n_kv) >= (1ll << 30))
     return qtb_fail(QTB_E_INVALID, "%lld requests, %lld tokens", (long long)d->n_req, (long long)d->n_tokens);
+  if (d->n_tokens / (TILE_M / (d->n_heads / d->n_kv)) + d->n_req >= (1ll << 31) / d->n_kv)   // units of work are counted in 32 bits
+    return qtb_fail(QTB_E_UNSUPPORTED, "%lld requests and %lld tokens over %lld key heads", (long long)d->n_req, (long long)d->n_tokens, (long long)d->n_kv);
   if (d->window < 0 || d->max_new < 0) return qtb_fail(QTB_E_INVALID, "window %lld, max_new %lld", (long long)d->window, (long long)d->max_new);
   if (!(d->scale == d->scale) || d->scale > 3e38 || d->scale < -3e38) return qtb_fail(QTB_E_INVALID, "scale is not finite");
   if (!d->cu_new || (d->n_tokens && (!d->q || !d->out)) || (d->n_tokens && !paged && (!d->k || !d->v)))
