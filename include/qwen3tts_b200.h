@@ -421,9 +421,10 @@ typedef struct {
     int64_t dtype, causal, window;
     double scale;
 } qtb_attn_t;
-/* Bytes of workspace for a call with these sizes (pointers are not read), or a
- * negative QTB_E_* code.  Its contents matter during one call only. */
-int64_t qtb_attn_workspace(const qtb_attn_t *d);
+/* Bytes of workspace for a call of the paged or the prompt form with these sizes,
+ * strides and scale (addresses matter for their alignment alone), or a negative QTB_E_* code.  Its
+ * contents matter during one call only. */
+int64_t qtb_attn_workspace(const qtb_attn_t *d, int paged);
 int qtb_paged_attention(const qtb_attn_t *d, void *stream);
 int qtb_prompt_attention(const qtb_attn_t *d, void *stream);
 

@@ -32,6 +32,7 @@
 #pragma once
 #include "qtb_paged.cuh"
 #include <cuda.h>
+#include <initializer_list>
 
 namespace qtb {
 
@@ -661,16 +662,25 @@ typedef CUresult (*TileEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t,
                                  const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+// Whether the call has a form that the tile kernel reads: a positive scale (its
+// maximum is taken before scaling) and tensors that TMA can describe (an expanded
+// axis, of stride 0, it cannot).  The others take the rows kernel.
+static inline bool tile_form(const AttnCall &c, bool paged) {
+  auto axis = [](long long ext, long long st) { return ext == 1 || st > 0; };
+  if (!(c.scale_log2 > 0.f) || !axis(c.n_heads, c.q_sh) || !axis(c.n_tokens, c.q_st)) return false;
+  for (const long long *st : {c.k_st, c.v_st}) {
+    if (paged && !(c.n_pages > 0 && axis(c.n_pages, st[0]) && axis(c.n_kv, st[1]) && axis(c.page, st[2]))) return false;
+    if (!paged && !(axis(c.n_tokens, st[0]) && axis(c.n_kv, st[1]))) return false;
+  }
+  return true;
+}
+
 // A tensor [d3][d2][d1][hd] (extents and strides of the outer axes, innermost
-// first) in boxes of [1][b2][b1][64] with the 128-byte swizzle.  False where TMA
-// cannot describe it (an expanded axis has stride 0).
+// first) in boxes of [1][b2][b1][64] with the 128-byte swizzle.
 static inline bool tile_map(TileEncodeFn fn, CUtensorMap *out, const void *base, bool f16, int hd, const long long (&ext)[3],
                             const long long (&st)[3], int b1, int b2) {
   cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)ext[0], (cuuint64_t)ext[1], (cuuint64_t)ext[2]}, bytes[3];
-  for (int i = 0; i < 3; i++) {
-    if (ext[i] < 1 || (ext[i] > 1 && st[i] <= 0)) return false;
-    bytes[i] = ext[i] > 1 ? (cuuint64_t)st[i] * 2 : (cuuint64_t)hd * 2;   // of an axis of one, any stride will do
-  }
+  for (int i = 0; i < 3; i++) bytes[i] = ext[i] > 1 ? (cuuint64_t)st[i] * 2 : (cuuint64_t)hd * 2;   // of an axis of one, any will do
   const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, one[4] = {1, 1, 1, 1};
   return fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, bytes,
             box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -684,12 +694,10 @@ static inline int tile_box(bool paged, int page) {
   return b;
 }
 
-// Whether the tensors have a form that the tile kernel reads, and its maps.
 static inline bool tile_maps(const AttnCall &c, bool paged, bool f16, int hd, TileEncodeFn fn, TileMaps &m) {
-  if (!fn || !(c.scale_log2 > 0.f)) return false;   // its maximum is taken before scaling
   const int tpt = TILE_M / c.group, box = tile_box(paged, c.page);
   const long long qe[3] = {c.n_heads, c.n_tokens, 1}, qs[3] = {c.q_sh, c.q_st, 0};
-  if (!tile_map(fn, &m.q, c.q, f16, hd, qe, qs, c.group, tpt)) return false;
+  if (!fn || !tile_map(fn, &m.q, c.q, f16, hd, qe, qs, c.group, tpt)) return false;
   if (paged) {
     const long long e[3] = {c.page, c.n_kv, c.n_pages};
     const long long ks[3] = {c.k_st[2], c.k_st[1], c.k_st[0]}, vs[3] = {c.v_st[2], c.v_st[1], c.v_st[0]};

@@ -315,6 +315,25 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
   return QTB_OK;
 }
 
+// Which kernel has a request goes by its query rows to a key head: few rows over
+// a long cache want the split key axis of the rows kernel, many rows the tiles;
+// prompts have no long cache.  max_new, where it is given, saves a launch.
+struct AttnPlan {
+  bool rows, tiles;
+  int limit;               // rows kernel: requests of at most so many rows
+};
+AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged) {
+  AttnPlan p;
+  p.tiles = tile_form(c, paged);
+  p.limit = !p.tiles ? INT_MAX : paged ? ROWS_M : 0;
+  if (p.tiles && paged && d->max_new > 0 && d->max_new * c.group <= ROWS_M) {
+    p.tiles = false;
+    p.limit = INT_MAX;
+  }
+  p.rows = p.limit > 0;
+  return p;
+}
+
 int attend(const qtb_attn_t *d, bool paged, void *stream) {
   AttnCall c;
   int rc = attn_call(d, paged, c);
@@ -322,20 +341,18 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   if (!c.n_req || !c.n_tokens) return QTB_OK;
   const DevInfo *dev;
   if ((rc = device_info(&dev))) return rc;
-  const int64_t need = qtb_attn_workspace(d);
-  if (need < 0) return (int)need;
+  const AttnPlan p = attn_plan(c, d, paged);
+  const int64_t need = p.rows ? (int64_t)rows_workspace((int)d->head_dim, dev->sms) : 0;
   if (d->workspace_bytes < need || (need && !d->workspace) || !aligned16(d->workspace))
     return qtb_fail(QTB_E_INVALID, "workspace of %lld bytes on 16: %lld needed", (long long)d->workspace_bytes, (long long)need);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == QTB_T_F16;
   const int hd = (int)d->head_dim;
   TileMaps maps;
-  const bool tiles = tile_maps(c, paged, f16, hd, dev->encode, maps);
-  // Which kernel has a request: few rows over a long cache want the split key
-  // axis of the rows kernel, many rows the tiles; prompts have no long cache.
-  const int limit = !tiles ? INT_MAX : paged ? ROWS_M : 0;
-  if (limit) PAGED_TRY(rows_launch(c, paged, f16, hd, dev->sms, limit, d->workspace, st));
-  if (tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, maps, dev->sms, limit, st));
+  if (p.tiles && !tile_maps(c, paged, f16, hd, dev->encode, maps))
+    return qtb_fail(QTB_E_UNSUPPORTED, "q, k or v have strides or extents that a tensor map cannot hold");
+  if (p.rows) PAGED_TRY(rows_launch(c, paged, f16, hd, dev->sms, p.limit, d->workspace, st));
+  if (p.tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, maps, dev->sms, p.limit, st));
   return QTB_OK;
 }
 
@@ -407,11 +424,13 @@ extern "C" int qtb_paged_append(const qtb_paged_append_t *d, void *stream) {
   return QTB_OK;
 }
 
-extern "C" int64_t qtb_attn_workspace(const qtb_attn_t *d) {
-  if (!d) return qtb_fail(QTB_E_INVALID, "null descriptor");
+extern "C" int64_t qtb_attn_workspace(const qtb_attn_t *d, int paged) {
+  AttnCall c;
+  if (int rc = attn_call(d, paged != 0, c)) return rc;
+  if (!c.n_req || !c.n_tokens) return 0;
   const DevInfo *dev;
   if (int rc = device_info(&dev)) return rc;
-  return rows_workspace((int)d->head_dim, dev->sms);
+  return paged || attn_plan(c, d, false).rows ? (int64_t)rows_workspace((int)d->head_dim, dev->sms) : 0;
 }
 
 extern "C" int qtb_paged_attention(const qtb_attn_t *d, void *stream) { return attend(d, true, stream); }
