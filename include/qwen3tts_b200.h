@@ -343,7 +343,7 @@ int qtb_attention_noalloc(const float *qkv, int batch, int n_heads, int n_kv, in
  * kernels check them there: what is out of range is not accessed, and the
  * reason is ORed into *status (NULL: not reported), which the caller zeroes.
  * Every field is 64 bits wide; strides are in elements, the innermost
- * dimension is contiguous, and tensor pointers and strides are multiples of 16
+ * dimension is contiguous, no axis is expanded (stride 0), and tensor pointers and strides are multiples of 16
  * bytes.  Nothing is read from tensors of extent zero. */
 enum {
     QTB_T_F32 = 0,

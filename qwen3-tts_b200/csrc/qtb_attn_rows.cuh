@@ -4,24 +4,32 @@
 // key head (token-major, the group's heads inside) are taken 16 at a time, the
 // M of mma.m16n8k16, so that grouped heads and the tokens of a short chunk read
 // K and V once.  Scores are in units of log2 (scale * log2 e folded in), and
-// each warp keeps the running maximum m, sum l and output O of its own keys:
-//   m' = max(m, s),  l' = l 2^(m - m') + sum 2^(s - m'),  O' likewise.
-// States of any two key sets join the same way, so the key axis is cut freely:
-// the (request, row group, key head, 64-key chunk) units of the whole call are
-// dealt out to the grid in equal runs, whatever the requests' lengths.  An item
-// that a block holds whole is written at once; one that is cut leaves its parts
-// (O, m, l in f32) in the workspace, and rows_join_kernel adds them in block
-// order, so results do not depend on timing.
+// each warp keeps a maximum m, the sum l of 2^(s - m) and the output O of its
+// own keys.  States of any two key sets join (m the larger, the other's l and O
+// scaled), so the key axis is cut freely: the (request, row group, key head,
+// 64-key chunk) units of the whole call are dealt out to the grid in equal
+// runs, whatever the requests' lengths.  An item that a block holds whole is
+// written at once; one that is cut leaves its parts (O, m, l in f32) in the
+// workspace, and rows_join_kernel adds them in block order, so results do not
+// depend on timing.
 //
-// Keys outside the request, pages outside the pool and rows past the request's
-// last are filled with zeros on the way to shared memory and their scores set
-// to -inf, so nothing that lies there (NaN, infinities) reaches a sum.
+// m is renewed lazily, when a score passes it by 2^8: until then the
+// probabilities are at most 2^8 and the quotient O / l does not care.
+//
+// What bounds it is the stream of K and V.  One warp copies by TMA (a box is a
+// run of a page's positions with all of its dims, 128-byte swizzle), four
+// compute; two blocks of three 64-key stages on an SM keep up to 192 KB in
+// flight.  Keys outside the request may hold anything: their scores become
+// -inf and their V is masked to zero in registers.
 #pragma once
 #include "qtb_paged.cuh"
+#include <cuda.h>
 
 namespace qtb {
 
-constexpr int ROWS_THREADS = 128, ROWS_WARPS = 4, ROWS_M = 16, ROWS_CHUNK = 64, ROWS_STAGES = 3, ROWS_PER_SM = 2;
+constexpr int ROWS_WARPS = 4, ROWS_THREADS = 32 * (ROWS_WARPS + 1), ROWS_M = 16, ROWS_CHUNK = 64, ROWS_PER_SM = 2;
+constexpr int ROWS_JOIN_WARPS = 8;
+constexpr long long ROWS_WAIT = 4000000000ll;   // cycles: about two seconds
 
 // Where a cut item's parts are, per block: the request, row group and head of
 // the item that the block starts and does not finish, and the last block that
@@ -29,13 +37,18 @@ constexpr int ROWS_THREADS = 128, ROWS_WARPS = 4, ROWS_M = 16, ROWS_CHUNK = 64, 
 struct RowsCut {
   int r, rg, h, last;
 };
+struct RowsMaps {
+  CUtensorMap k, v;
+};
 
 template <int HD>
 constexpr int rows_part_floats() { return ROWS_M * (HD + 2); }   // O rows, then (m, l) pairs
 template <int HD>
-constexpr int rows_smem() {
-  return ROWS_STAGES * 2 * ROWS_CHUNK * HD * 2 + 2 * 32 * (HD / 2) * 4 + ROWS_WARPS * ROWS_M * 2 * 4;
-}
+constexpr int rows_stages() { return HD == 128 ? 3 : 6; }
+template <int HD>
+constexpr int rows_keys_bytes() { return ROWS_CHUNK * HD * 2; }
+template <int HD>
+constexpr int rows_smem() { return rows_stages<HD>() * 2 * rows_keys_bytes<HD>() + 2 * 32 * (HD / 2) * 4; }
 
 // A position in the call's sequence of units.
 template <bool PAGED>
@@ -67,24 +80,35 @@ struct RowsCursor {
   }
 };
 
+struct RowsShared {
+  uint64_t full[8], empty[8];
+  long long sum[ROWS_WARPS + 1], off;      // off: the first unit's index within its request
+  int req, abort;
+  float2 ml[ROWS_WARPS][ROWS_M];
+};
+
 template <int HD, bool F16, bool PAGED>
 __global__ void __launch_bounds__(ROWS_THREADS, ROWS_PER_SM)
-rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut *__restrict__ cuts) {
+rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_limit, int box, float *__restrict__ parts,
+            RowsCut *__restrict__ cuts) {
   constexpr int KS = HD / 16;              // k-steps of Q K^T
   constexpr int NT = HD / 8;               // 8-wide output tiles
-  constexpr int UPR = HD / 8;              // 16-byte units of a key row
-  constexpr int PASS_ROWS = ROWS_THREADS / UPR, PASSES = ROWS_CHUNK / PASS_ROWS;
-  constexpr int KEYS_B = ROWS_CHUNK * HD * 2;
-  extern __shared__ __align__(128) unsigned char smem[];
-  float *s_red = reinterpret_cast<float *>(smem + ROWS_STAGES * 2 * KEYS_B);   // [2][HD / 2][32]
-  float2 *s_ml = reinterpret_cast<float2 *>(s_red + 2 * 32 * (HD / 2));        // [warp][16] (m, l)
-  __shared__ long long s_sum[ROWS_WARPS];
-  __shared__ long long s_off;              // first unit's index within its request
-  __shared__ int s_req;
+  constexpr int STAGES = rows_stages<HD>(), KEYS_B = rows_keys_bytes<HD>();
+  extern __shared__ __align__(1024) unsigned char rows_smem_base[];
+  unsigned char *smem = rows_smem_base;
+  float *s_red = reinterpret_cast<float *>(smem + STAGES * 2 * KEYS_B);   // [2][HD / 2][32]
+  __shared__ RowsShared sh;
 
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gid = lane >> 2, tig = lane & 3;
+  const int tid = threadIdx.x, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
+  const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
+  pdl_release();                           // the join kernel's blocks may come up; they wait for this grid's end
 
-  // --- this block's run of units: thread i counts requests [i n / 128, (i + 1) n / 128)
+  // --- this block's run of units: thread i counts requests [i n / 160, (i + 1) n / 160)
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; i++) { mbar_init(&sh.full[i], 1); mbar_init(&sh.empty[i], ROWS_WARPS); }
+    sh.abort = 0;
+    fence_mbar_init();
+  }
   RowsCursor<PAGED> cur;
   const int ra = (int)((long long)c.n_req * tid / ROWS_THREADS), rb = (int)((long long)c.n_req * (tid + 1) / ROWS_THREADS);
   long long sum = 0;
@@ -98,13 +122,13 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
     const long long x = __shfl_up_sync(0xffffffffu, pre, o);
     if (lane >= o) pre += x;
   }
-  if (lane == 31) s_sum[warp] = pre;
+  if (lane == 31) sh.sum[warp] = pre;
   __syncthreads();
   long long total = 0;
 #pragma unroll
-  for (int w = 0; w < ROWS_WARPS; w++) {
-    if (w < warp) pre += s_sum[w];
-    total += s_sum[w];
+  for (int w = 0; w <= ROWS_WARPS; w++) {
+    if (w < warp) pre += sh.sum[w];
+    total += sh.sum[w];
   }
   pre -= sum;
   const long long blocks = min((long long)gridDim.x, total);
@@ -119,65 +143,96 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
       if (u0 < at + n) break;
       at += n;
     }
-    s_req = cur.r;
-    s_off = u0 - at;
+    sh.req = cur.r;
+    sh.off = u0 - at;
   }
   __syncthreads();
-  cur.r = s_req;
+  cur.r = sh.req;
   cur.load(c, row_limit);
   {
-    long long off = s_off;
-    cur.ch = (int)(off % cur.chunks);
-    off /= cur.chunks;
-    cur.h = (int)(off % c.n_kv);
-    cur.rg = (int)(off / c.n_kv);
+    unsigned long long off = (unsigned long long)sh.off;
+    cur.ch = (int)(off % (unsigned)cur.chunks);
+    off /= (unsigned)cur.chunks;
+    cur.h = (int)(off % (unsigned)c.n_kv);
+    cur.rg = (int)(off / (unsigned)c.n_kv);
   }
-  RowsCursor<PAGED> ld = cur;              // runs ahead of `cur` by the copies in flight
-  int bad = 0;
+  const int n_units = (int)(u1 - u0);
 
-  auto copy_unit = [&](int stage) {
-    unsigned char *ks = smem + stage * 2 * KEYS_B, *vs = ks + KEYS_B;
-    const int row0 = tid / UPR, unit = tid % UPR, pos0 = (ld.c0 + ld.ch) * ROWS_CHUNK;
-#pragma unroll
-    for (int p = 0; p < PASSES; p++) {
-      const int row = p * PASS_ROWS + row0, pos = pos0 + row;
-      bool ok = pos >= ld.a.lo && pos < ld.a.hi;
-      const uint16_t *kp = c.k, *vp = c.v;
-      if (ok) {
-        if (PAGED) {
-          const int e = pos / c.page, pg = c.table[ld.r * c.table_stride + e];
-          if (pg < 0 || pg >= c.n_pages) { ok = false; bad |= QTB_PS_PAGE; }
-          else {
-            const long long off = pos - e * c.page;
-            kp += pg * c.k_st[0] + ld.h * c.k_st[1] + off * c.k_st[2] + unit * 8;
-            vp += pg * c.v_st[0] + ld.h * c.v_st[1] + off * c.v_st[2] + unit * 8;
-          }
-        } else {
-          const long long t = ld.a.t0 + pos;
-          kp += t * c.k_st[0] + ld.h * c.k_st[1] + unit * 8;
-          vp += t * c.v_st[0] + ld.h * c.v_st[1] + unit * 8;
-        }
+  // Bounded wait; one that runs out lets the block run on without data, so that
+  // its own barriers are met, and reports it.
+  auto wait = [&](uint64_t *bar, uint32_t parity) {
+    if (mbar_wait(bar, parity, 20000)) return true;
+    const long long t0 = clock64();
+    while (!*reinterpret_cast<volatile int *>(&sh.abort)) {
+      if (mbar_wait(bar, parity, 20000)) return true;
+      if (clock64() - t0 > ROWS_WAIT) {
+        *reinterpret_cast<volatile int *>(&sh.abort) = 1;
+        raise_status(c.status, QTB_PS_TIMEOUT);
       }
-      const int at = row * (HD * 2) + ((unit ^ (row & 7)) << 4);
-      cp16_zfill(ks + at, kp, ok);
-      cp16_zfill(vs + at, vp, ok);
     }
+    return false;
   };
 
-  const long long n_units = u1 - u0;
-#pragma unroll
-  for (int s = 0; s < ROWS_STAGES - 1; s++) {
-    if (s < n_units) { copy_unit(s); ld.next(c, row_limit); }
-    cp_commit();
+  if (warp == ROWS_WARPS) {
+    // ------------------------------------------------------------- loads ---
+    // Lanes 0-3 have the chunk's boxes of K, lanes 4-7 of V.
+    const int boxes = ROWS_CHUNK / box, bi = lane & 3, kv = (lane >> 2) & 1;
+    const uint32_t bytes = (uint32_t)(box * HD * 2);
+    unsigned char *dst0 = smem + kv * KEYS_B + bi * bytes;
+    const CUtensorMap *map = kv ? &maps.v : &maps.k;
+    int bad = 0, u = 0, pg = 0, off = 0;
+    bool mine = false;
+    auto find = [&]() {                    // this lane's box of the cursor's chunk
+      const int pos = (cur.c0 + cur.ch) * ROWS_CHUNK + bi * box;
+      mine = lane < 8 && bi < boxes && pos < cur.a.hi && pos + box > cur.a.lo;
+      if (PAGED) {
+        if (mine) {
+          const int e = pos / c.page;
+          off = pos - e * c.page;
+          pg = c.table[cur.r * c.table_stride + e];
+        }
+      } else {
+        off = cur.a.t0 + pos;
+      }
+    };
+    find();
+    for (; u < n_units; u++) {
+      const int st = u % STAGES;
+      if (!__all_sync(0xffffffffu, wait(&sh.empty[st], ((u / STAGES) & 1) ^ 1))) break;
+      const int count = __popc(__ballot_sync(0xffffffffu, mine));
+      if (lane == 0) mbar_arrive_expect_tx(&sh.full[st], (uint32_t)count * bytes);
+      __syncwarp();
+      if (mine) {
+        if (PAGED && (pg < 0 || pg >= c.n_pages)) { pg = c.n_pages; bad = QTB_PS_PAGE; }   // past the last page: zeros
+        tma_load_5d(dst0 + st * 2 * KEYS_B, map, 0, off, 0, cur.h, PAGED ? pg : 0, &sh.full[st]);
+      }
+      cur.next(c, row_limit);
+      if (u + 1 < n_units) find();
+    }
+    // copies in flight land before the block leaves
+    for (int f = max(u - STAGES, 0); f < u; f++) mbar_wait(&sh.full[f % STAGES], (f / STAGES) & 1, ROWS_WAIT);
+    raise_status(c.status, bad);
+    return;
   }
+
+  // ----------------------------------------------------------------- math ---
+  const float scale = fabsf(c.scale_log2);
+  const uint32_t flip = c.scale_log2 < 0.f ? 0x80008000u : 0u;   // a negative scale turns the queries' signs
+  const uint32_t keep = c.scale_log2 == 0.f ? 0u : 0xffffffffu;  // a scale of zero makes them zeros ...
+  const float mul = c.scale_log2 == 0.f ? 1.f : scale;           // ... so that -inf stays -inf
+  // this warp's 16 keys within a stage: [box][half][row][128 bytes]
+  const int half_b = box * 128;
+  const int k_at = (warp * 16 / box) * half_b * (HD / 64) + (warp * 16 % box) * 128;
+  const int k_row = (lane & 7) + ((lane & 16) >> 1), k_half = (lane >> 3) & 1, v_row = lane & 15, v_half = lane >> 4;
 
   uint32_t q[KS][4];
   float o[NT][4], m[2], l[2];
   int last_key[2], first_key[2], tok[2];   // per row: the keys it sees, its token (-1: no row)
+  int all_first = 0, all_last = 0;         // keys that every row sees
   bool starts = cur.ch == 0;               // this block holds the current item from its first chunk
   bool fresh = true;
 
-  for (long long u = 0; u < n_units; u++) {
+  for (int u = 0; u < n_units; u++) {
     if (fresh) {
       fresh = false;
 #pragma unroll
@@ -185,63 +240,62 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
         const int row = cur.rg * ROWS_M + gid + 8 * i, t = row / c.group, g = row - t * c.group;
         const bool live = t < cur.a.n;
         tok[i] = live ? t : -1;
-        last_key[i] = !live ? -1 : c.causal ? cur.a.first + t : cur.a.hi - 1;
+        last_key[i] = !live ? -1 : min(c.causal ? cur.a.first + t : cur.a.hi - 1, cur.a.hi - 1);
         first_key[i] = c.window > 0 ? max(cur.a.first + t - c.window + 1, 0) : 0;
         const uint16_t *qp = c.q + (long long)(cur.a.t0 + t) * c.q_st + (long long)(cur.h * c.group + g) * c.q_sh + 2 * tig;
 #pragma unroll
         for (int k = 0; k < KS; k++) {
-          q[k][i] = live ? __ldg(reinterpret_cast<const uint32_t *>(qp + 16 * k)) : 0u;
-          q[k][2 + i] = live ? __ldg(reinterpret_cast<const uint32_t *>(qp + 16 * k + 8)) : 0u;
+          q[k][i] = live ? (__ldg(reinterpret_cast<const uint32_t *>(qp + 16 * k)) ^ flip) & keep : 0u;
+          q[k][2 + i] = live ? (__ldg(reinterpret_cast<const uint32_t *>(qp + 16 * k + 8)) ^ flip) & keep : 0u;
         }
         m[i] = -INFINITY;
         l[i] = 0.f;
       }
+      const int t_a = cur.rg * ROWS_M / c.group, t_b = min((cur.rg * ROWS_M + ROWS_M - 1) / c.group, cur.a.n - 1);
+      all_last = min(c.causal ? cur.a.first + t_a : cur.a.hi - 1, cur.a.hi - 1);
+      all_first = c.window > 0 ? max(cur.a.first + t_b - c.window + 1, 0) : 0;
 #pragma unroll
       for (int n = 0; n < NT; n++)
 #pragma unroll
         for (int i = 0; i < 4; i++) o[n][i] = 0.f;
     }
-    cp_wait<ROWS_STAGES - 2>();
-    __syncthreads();
-    if (u + ROWS_STAGES - 1 < n_units) {
-      copy_unit((int)((u + ROWS_STAGES - 1) % ROWS_STAGES));
-      ld.next(c, row_limit);
-    }
-    cp_commit();
+    const int st = u % STAGES;
+    wait(&sh.full[st], (u / STAGES) & 1);
+    __syncwarp();
 
     // --- this warp's 16 keys of the chunk
-    const unsigned char *ks = smem + (int)(u % ROWS_STAGES) * 2 * KEYS_B, *vs = ks + KEYS_B;
+    const unsigned char *ks = smem + st * 2 * KEYS_B + k_at, *vs = ks + KEYS_B;
     const int key0 = (cur.c0 + cur.ch) * ROWS_CHUNK + warp * 16;
     float s[2][4] = {};
-    {
-      const int row = warp * 16 + (lane & 7) + ((lane & 16) >> 1), half = (lane >> 3) & 1;
 #pragma unroll
-      for (int k = 0; k < KS; k++) {
-        uint32_t b[4];
-        ldsm_x4(b, ks + row * (HD * 2) + (((2 * k + half) ^ (row & 7)) << 4));
-        mma16<F16>(s[0], q[k], b[0], b[1]);
-        mma16<F16>(s[1], q[k], b[2], b[3]);
+    for (int k = 0; k < KS; k++) {
+      uint32_t b[4];
+      ldsm_x4(b, ks + (k >> 2) * half_b + k_row * 128 + ((((2 * k) & 7) + k_half) ^ (k_row & 7)) * 16);
+      mma16<F16>(s[0], q[k], b[0], b[1]);
+      mma16<F16>(s[1], q[k], b[2], b[3]);
+    }
+    uint32_t vmask[2] = {0xffffffffu, 0xffffffffu};   // of keys 2 tig, 2 tig + 1 and those 8 on
+    if (key0 < all_first || key0 + 15 > all_last) {
+#pragma unroll
+      for (int t = 0; t < 2; t++) {
+        const int key = key0 + 8 * t + 2 * tig;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (key + (i & 1) > last_key[i >> 1] || key + (i & 1) < first_key[i >> 1]) s[t][i] = -INFINITY;
+        vmask[t] = (key >= cur.a.lo && key < cur.a.hi ? 0xffffu : 0u) | (key + 1 >= cur.a.lo && key + 1 < cur.a.hi ? 0xffff0000u : 0u);
       }
     }
-    float mx[2] = {m[0], m[1]};
+    float mx[2];
 #pragma unroll
-    for (int t = 0; t < 2; t++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const int key = key0 + 8 * t + 2 * tig + (i & 1), w = i >> 1;
-        s[t][i] = key <= last_key[w] && key >= first_key[w] ? s[t][i] * c.scale_log2 : -INFINITY;
-        mx[w] = fmaxf(mx[w], s[t][i]);
-      }
-#pragma unroll
-    for (int w = 0; w < 2; w++) {
-      mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 1));
-      mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 2));
-    }
-    if (__any_sync(0xffffffffu, mx[0] != m[0] || mx[1] != m[1])) {
+    for (int w = 0; w < 2; w++)
+      mx[w] = fmaxf(fmaxf(s[0][2 * w], s[0][2 * w + 1]), fmaxf(s[1][2 * w], s[1][2 * w + 1])) * mul;
+    if (__any_sync(0xffffffffu, mx[0] > m[0] + 8.f || mx[1] > m[1] + 8.f)) {
 #pragma unroll
       for (int w = 0; w < 2; w++) {
-        const float f = mx[w] == -INFINITY ? 1.f : exp2_approx(m[w] - mx[w]);
-        m[w] = mx[w];
+        mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 1));
+        mx[w] = fmaxf(mx[w], __shfl_xor_sync(0xffffffffu, mx[w], 2));
+        const float m2 = fmaxf(m[w], mx[w]), f = m2 == -INFINITY ? 1.f : exp2_approx(m[w] - m2);
+        m[w] = m2;
         l[w] *= f;
 #pragma unroll
         for (int n = 0; n < NT; n++) { o[n][2 * w] *= f; o[n][2 * w + 1] *= f; }
@@ -252,23 +306,22 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
     for (int t = 0; t < 2; t++)
 #pragma unroll
       for (int i = 0; i < 4; i++) {
-        s[t][i] = exp2_approx(s[t][i] - base[i >> 1]);
+        s[t][i] = exp2_approx(fmaf(s[t][i], mul, -base[i >> 1]));
         l[i >> 1] += s[t][i];
       }
     // probabilities are rounded to the cache's type for the product with V, as
     // large as the result's own rounding; their sum l is of the unrounded ones
     const uint32_t pa[4] = {pack2<F16>(s[0][0], s[0][1]), pack2<F16>(s[0][2], s[0][3]),
                             pack2<F16>(s[1][0], s[1][1]), pack2<F16>(s[1][2], s[1][3])};
-    {
-      const int row = warp * 16 + (lane & 15), half = lane >> 4;
 #pragma unroll
-      for (int n = 0; n < NT; n += 2) {
-        uint32_t b[4];
-        ldsm_x4_trans(b, vs + row * (HD * 2) + (((n + half) ^ (row & 7)) << 4));
-        mma16<F16>(o[n], pa, b[0], b[1]);
-        mma16<F16>(o[n + 1], pa, b[2], b[3]);
-      }
+    for (int n = 0; n < NT; n += 2) {
+      uint32_t b[4];
+      ldsm_x4_trans(b, vs + (n >> 3) * half_b + v_row * 128 + (((n & 7) + v_half) ^ (v_row & 7)) * 16);
+      mma16<F16>(o[n], pa, b[0] & vmask[0], b[1] & vmask[1]);
+      mma16<F16>(o[n + 1], pa, b[2] & vmask[0], b[3] & vmask[1]);
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&sh.empty[st]);
 
     const bool ends = cur.ch == cur.chunks - 1;
     if (ends || u + 1 == n_units) {
@@ -277,20 +330,20 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
       for (int w = 0; w < 2; w++) {
         l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
         l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
-        if (tig == 0) s_ml[warp * ROWS_M + gid + 8 * w] = make_float2(m[w], l[w]);
+        if (tig == 0) sh.ml[warp][gid + 8 * w] = make_float2(m[w], l[w]);
       }
-      __syncthreads();
+      bar_sync_n(1, 32 * ROWS_WARPS);
       float mt[2], lt[2];
 #pragma unroll
       for (int w = 0; w < 2; w++) {
         mt[w] = -INFINITY;
         lt[w] = 0.f;
 #pragma unroll
-        for (int i = 0; i < ROWS_WARPS; i++) mt[w] = fmaxf(mt[w], s_ml[i * ROWS_M + gid + 8 * w].x);
+        for (int i = 0; i < ROWS_WARPS; i++) mt[w] = fmaxf(mt[w], sh.ml[i][gid + 8 * w].x);
         const float b = mt[w] == -INFINITY ? 0.f : mt[w];
 #pragma unroll
         for (int i = 0; i < ROWS_WARPS; i++) {
-          const float2 x = s_ml[i * ROWS_M + gid + 8 * w];
+          const float2 x = sh.ml[i][gid + 8 * w];
           lt[w] += x.y * exp2_approx(x.x - b);
         }
         const float f = exp2_approx(m[w] - b);
@@ -306,7 +359,7 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
 #pragma unroll
             for (int i = 0; i < 4; i++) d[(n * 4 + i) * 32 + lane] = o[n][i];
         }
-        __syncthreads();
+        bar_sync_n(1, 32 * ROWS_WARPS);
         if (warp < half) {
           const float *d = s_red + warp * 32 * (HD / 2);
 #pragma unroll
@@ -314,7 +367,7 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
 #pragma unroll
             for (int i = 0; i < 4; i++) o[n][i] += d[(n * 4 + i) * 32 + lane];
         }
-        __syncthreads();
+        bar_sync_n(1, 32 * ROWS_WARPS);
       }
       if (warp == 0) {
         if (starts && ends) {
@@ -336,6 +389,7 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
           float *d = parts + (long long)(2 * blockIdx.x + (starts ? 1 : 0)) * rows_part_floats<HD>();
 #pragma unroll
           for (int w = 0; w < 2; w++) {
+            if (tok[w] < 0) continue;
             const int row = gid + 8 * w;
 #pragma unroll
             for (int n = 0; n < NT; n++)
@@ -356,38 +410,57 @@ rows_kernel(const AttnCall c, int row_limit, float *__restrict__ parts, RowsCut 
     }
     cur.next(c, row_limit);
   }
-  cp_wait<0>();
-  raise_status(c.status, bad);
 }
 
 // Joins the parts of the item that block blockIdx.x cut: part 1 of that block,
-// then part 0 of the following ones, in that order.
+// then part 0 of the following ones, in that order.  A warp has a row, a lane
+// HD / 32 of its dims.
 template <int HD, bool F16, bool PAGED>
-__global__ void __launch_bounds__(HD)
+__global__ void __launch_bounds__(32 * ROWS_JOIN_WARPS)
 rows_join_kernel(const AttnCall c, const float *__restrict__ parts, const RowsCut *__restrict__ cuts) {
+  constexpr int PF = rows_part_floats<HD>(), V = HD / 32, UNROLL = 8;
   pdl_wait();
   const RowsCut cut = cuts[blockIdx.x];
   if (cut.last < 0) return;
   const AttnReq a = attn_request<PAGED>(c, cut.r);
-  const int d = threadIdx.x, b0 = blockIdx.x;
-  constexpr int PF = rows_part_floats<HD>();
-  auto part = [&](int b) { return parts + (long long)(2 * b + (b == b0 ? 1 : 0)) * PF; };
-  for (int i = 0; i < ROWS_M; i++) {
-    const int row = cut.rg * ROWS_M + i, t = row / c.group, h = cut.h * c.group + row - t * c.group;
+  const int lane = threadIdx.x & 31, b0 = blockIdx.x, n = cut.last - b0 + 1;
+  auto part = [&](int i) { return parts + (long long)(2 * (b0 + i) + (i == 0 ? 1 : 0)) * PF; };
+  for (int row = threadIdx.x >> 5; row < ROWS_M; row += ROWS_JOIN_WARPS) {
+    const int rr = cut.rg * ROWS_M + row, t = rr / c.group, h = cut.h * c.group + rr - t * c.group;
     if (t >= a.n) return;
     float m = -INFINITY;
-    for (int b = b0; b <= cut.last; b++) m = fmaxf(m, part(b)[ROWS_M * HD + 2 * i]);
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, part(i)[ROWS_M * HD + 2 * row]);
+    m = warp_max(m);
     const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o = 0.f;
-    for (int b = b0; b <= cut.last; b++) {
-      const float *p = part(b), f = exp2_approx(p[ROWS_M * HD + 2 * i] - base);
-      l += p[ROWS_M * HD + 2 * i + 1] * f;
-      o += p[i * HD + d] * f;
+    float l = 0.f, o[V] = {};
+    for (int i0 = 0; i0 < n; i0 += UNROLL) {
+      float x[UNROLL][V], f[UNROLL], z[UNROLL];
+#pragma unroll
+      for (int i = 0; i < UNROLL; i++) {
+        const float *p = part(min(i0 + i, n - 1));
+#pragma unroll
+        for (int v = 0; v < V; v += 2) {
+          const float2 y = *reinterpret_cast<const float2 *>(p + row * HD + V * lane + v);
+          x[i][v] = y.x; x[i][v + 1] = y.y;
+        }
+        f[i] = p[ROWS_M * HD + 2 * row];
+        z[i] = p[ROWS_M * HD + 2 * row + 1];
+      }
+#pragma unroll
+      for (int i = 0; i < UNROLL; i++) {
+        if (i0 + i >= n) break;
+        const float w = exp2_approx(f[i] - base);
+        l += z[i] * w;
+#pragma unroll
+        for (int v = 0; v < V; v++) o[v] += x[i][v] * w;
+      }
     }
     const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
     const long long at = a.t0 + t;
-    c.out[at * c.o_st + h * c.o_sh + d] = (uint16_t)pack2<F16>(o * inv, 0.f);
-    if (c.lse && d == 0) c.lse[at * c.n_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    uint16_t *op = c.out + at * c.o_st + h * c.o_sh + V * lane;
+#pragma unroll
+    for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t *>(op + v) = pack2<F16>(o[v] * inv, o[v + 1] * inv);
+    if (c.lse && lane == 0) c.lse[at * c.n_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
 }
 
@@ -397,50 +470,66 @@ static inline size_t rows_workspace(int hd, int sms) {
   return grid * 16 + grid * 2 * (size_t)(hd == 128 ? rows_part_floats<128>() : rows_part_floats<64>()) * 4;
 }
 
-template <int HD, bool F16, bool PAGED>
-static cudaError_t rows_prepare_one() {
-  return cudaFuncSetAttribute(rows_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem<HD>());
+// Keys in boxes of a run of a page's positions, all dims: [dim / 64][position][64].
+static inline int rows_box(bool paged, int page) {
+  int b = ROWS_CHUNK;
+  while (paged && page % b) b >>= 1;
+  return b;
 }
-static inline cudaError_t rows_prepare() {
-  cudaError_t e;
-  if ((e = rows_prepare_one<128, false, false>()) != cudaSuccess) return e;
-  if ((e = rows_prepare_one<128, false, true>()) != cudaSuccess) return e;
-  if ((e = rows_prepare_one<128, true, false>()) != cudaSuccess) return e;
-  if ((e = rows_prepare_one<128, true, true>()) != cudaSuccess) return e;
-  if ((e = rows_prepare_one<64, false, false>()) != cudaSuccess) return e;
-  if ((e = rows_prepare_one<64, false, true>()) != cudaSuccess) return e;
-  if ((e = rows_prepare_one<64, true, false>()) != cudaSuccess) return e;
-  return rows_prepare_one<64, true, true>();
+static inline bool rows_maps(const AttnCall &c, bool paged, bool f16, int hd, TensorMapFn fn, RowsMaps &m) {
+  const long long pos = paged ? c.page : c.n_tokens, pages = paged ? c.n_pages : 1;
+  auto one = [&](CUtensorMap *out, const uint16_t *base, const long long *st) {
+    const long long ext[5] = {64, pos, hd / 64, c.n_kv, pages};
+    const long long str[5] = {1, paged ? st[2] : st[0], 64, st[1], paged ? st[0] : 0};
+    const int box[5] = {64, rows_box(paged, c.page), hd / 64, 1, 1};
+    return tensor_map(fn, out, base, f16, 5, ext, str, box);
+  };
+  return one(&m.k, c.k, c.k_st) && one(&m.v, c.v, c.v_st);
 }
 
 template <int HD, bool F16, bool PAGED>
-static cudaError_t rows_launch_one(const AttnCall &c, int sms, int row_limit, void *ws, cudaStream_t st) {
+static cudaError_t rows_run(bool prepare, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, void *ws, cudaStream_t st) {
+  if (prepare)
+    return cudaFuncSetAttribute(rows_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem<HD>());
   const int grid = sms * ROWS_PER_SM;
   RowsCut *cuts = static_cast<RowsCut *>(ws);
   float *parts = reinterpret_cast<float *>(static_cast<char *>(ws) + (size_t)grid * sizeof(RowsCut));
-  rows_kernel<HD, F16, PAGED><<<grid, ROWS_THREADS, rows_smem<HD>(), st>>>(c, row_limit, parts, cuts);
+  rows_kernel<HD, F16, PAGED><<<grid, ROWS_THREADS, rows_smem<HD>(), st>>>(*c, *m, row_limit, rows_box(PAGED, c->page), parts, cuts);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
   cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(HD);
+  cfg.blockDim = dim3(32 * ROWS_JOIN_WARPS);
   cfg.stream = st;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, rows_join_kernel<HD, F16, PAGED>, c, (const float *)parts, (const RowsCut *)cuts);
+  return cudaLaunchKernelEx(&cfg, rows_join_kernel<HD, F16, PAGED>, *c, (const float *)parts, (const RowsCut *)cuts);
 }
 // Requests with at most row_limit query rows to a key head are served.
-static inline cudaError_t rows_launch(const AttnCall &c, bool paged, bool f16, int hd, int sms, int row_limit, void *ws,
-                                      cudaStream_t st) {
-  if (hd == 128) {
-    if (f16) return paged ? rows_launch_one<128, true, true>(c, sms, row_limit, ws, st) : rows_launch_one<128, true, false>(c, sms, row_limit, ws, st);
-    return paged ? rows_launch_one<128, false, true>(c, sms, row_limit, ws, st) : rows_launch_one<128, false, false>(c, sms, row_limit, ws, st);
+static inline cudaError_t rows_any(bool prepare, int which, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, void *ws,
+                                   cudaStream_t st) {
+  switch (which) {
+    case 0: return rows_run<64, false, false>(prepare, c, m, sms, row_limit, ws, st);
+    case 1: return rows_run<64, false, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 2: return rows_run<64, true, false>(prepare, c, m, sms, row_limit, ws, st);
+    case 3: return rows_run<64, true, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 4: return rows_run<128, false, false>(prepare, c, m, sms, row_limit, ws, st);
+    case 5: return rows_run<128, false, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 6: return rows_run<128, true, false>(prepare, c, m, sms, row_limit, ws, st);
+    default: return rows_run<128, true, true>(prepare, c, m, sms, row_limit, ws, st);
   }
-  if (f16) return paged ? rows_launch_one<64, true, true>(c, sms, row_limit, ws, st) : rows_launch_one<64, true, false>(c, sms, row_limit, ws, st);
-  return paged ? rows_launch_one<64, false, true>(c, sms, row_limit, ws, st) : rows_launch_one<64, false, false>(c, sms, row_limit, ws, st);
+}
+static inline cudaError_t rows_prepare() {
+  for (int i = 0; i < 8; i++)
+    if (cudaError_t e = rows_any(true, i, nullptr, nullptr, 0, 0, nullptr, nullptr)) return e;
+  return cudaSuccess;
+}
+static inline cudaError_t rows_launch(const AttnCall &c, bool paged, bool f16, int hd, const RowsMaps &m, int sms, int row_limit,
+                                      void *ws, cudaStream_t st) {
+  return rows_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, row_limit, ws, st);
 }
 
 }  // namespace qtb

@@ -31,8 +31,6 @@
 // leave.
 #pragma once
 #include "qtb_paged.cuh"
-#include <cuda.h>
-#include <initializer_list>
 
 namespace qtb {
 
@@ -124,16 +122,6 @@ template <int N>
 QTB_DEV void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 QTB_DEV void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-QTB_DEV void mbar_arrive(uint64_t *bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-QTB_DEV void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
-          smem_u32(dst)),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
-      : "memory");
-}
 // Whether the phase has completed, after waiting a short while for it.
 QTB_DEV bool mbar_try(uint64_t *bar, uint32_t parity) {
   uint32_t done;
@@ -195,10 +183,10 @@ __global__ void __launch_bounds__(TILE_THREADS, 1)
 tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int tpt, int box) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
-  extern __shared__ __align__(1024) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char tile_smem_base[];
+  unsigned char *smem = tile_smem_base;
   TileShared &sh = *reinterpret_cast<TileShared *>(smem + tile_operands<HD>());
   TileSync &sy = sh.sy;
-  int *s_pre = sh.pre;
   unsigned char *s_q = smem, *s_kv = smem + 2 * Q_B;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // known to be the same in the whole warp
@@ -658,34 +646,9 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
 }
 
 // ------------------------------------------------------------------ host ---
-typedef CUresult (*TileEncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
-                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-// Whether the call has a form that the tile kernel reads: a positive scale (its
-// maximum is taken before scaling) and tensors that TMA can describe (an expanded
-// axis, of stride 0, it cannot).  The others take the rows kernel.
-static inline bool tile_form(const AttnCall &c, bool paged) {
-  auto axis = [](long long ext, long long st) { return ext == 1 || st > 0; };
-  if (!(c.scale_log2 > 0.f) || !axis(c.n_heads, c.q_sh) || !axis(c.n_tokens, c.q_st)) return false;
-  for (const long long *st : {c.k_st, c.v_st}) {
-    if (paged && !(c.n_pages > 0 && axis(c.n_pages, st[0]) && axis(c.n_kv, st[1]) && axis(c.page, st[2]))) return false;
-    if (!paged && !(axis(c.n_tokens, st[0]) && axis(c.n_kv, st[1]))) return false;
-  }
-  return true;
-}
-
-// A tensor [d3][d2][d1][hd] (extents and strides of the outer axes, innermost
-// first) in boxes of [1][b2][b1][64] with the 128-byte swizzle.
-static inline bool tile_map(TileEncodeFn fn, CUtensorMap *out, const void *base, bool f16, int hd, const long long (&ext)[3],
-                            const long long (&st)[3], int b1, int b2) {
-  cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)ext[0], (cuuint64_t)ext[1], (cuuint64_t)ext[2]}, bytes[3];
-  for (int i = 0; i < 3; i++) bytes[i] = ext[i] > 1 ? (cuuint64_t)st[i] * 2 : (cuuint64_t)hd * 2;   // of an axis of one, any will do
-  const cuuint32_t box[4] = {64, (cuuint32_t)b1, (cuuint32_t)b2, 1}, one[4] = {1, 1, 1, 1};
-  return fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(base), dims, bytes,
-            box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
+// Whether the tile kernel can have the call: it takes the maximum of the scores
+// before they are scaled.
+static inline bool tile_form(const AttnCall &c) { return c.scale_log2 > 0.f; }
 
 // The key box: as many of a page's positions as divide both page and tile.
 static inline int tile_box(bool paged, int page) {
@@ -694,18 +657,15 @@ static inline int tile_box(bool paged, int page) {
   return b;
 }
 
-static inline bool tile_maps(const AttnCall &c, bool paged, bool f16, int hd, TileEncodeFn fn, TileMaps &m) {
-  const int tpt = TILE_M / c.group, box = tile_box(paged, c.page);
-  const long long qe[3] = {c.n_heads, c.n_tokens, 1}, qs[3] = {c.q_sh, c.q_st, 0};
-  if (!fn || !tile_map(fn, &m.q, c.q, f16, hd, qe, qs, c.group, tpt)) return false;
-  if (paged) {
-    const long long e[3] = {c.page, c.n_kv, c.n_pages};
-    const long long ks[3] = {c.k_st[2], c.k_st[1], c.k_st[0]}, vs[3] = {c.v_st[2], c.v_st[1], c.v_st[0]};
-    return tile_map(fn, &m.k, c.k, f16, hd, e, ks, box, 1) && tile_map(fn, &m.v, c.v, f16, hd, e, vs, box, 1);
-  }
-  const long long e[3] = {c.n_tokens, c.n_kv, 1};
-  const long long ks[3] = {c.k_st[0], c.k_st[1], 0}, vs[3] = {c.v_st[0], c.v_st[1], 0};
-  return tile_map(fn, &m.k, c.k, f16, hd, e, ks, box, 1) && tile_map(fn, &m.v, c.v, f16, hd, e, vs, box, 1);
+static inline bool tile_maps(const AttnCall &c, bool paged, bool f16, int hd, TensorMapFn fn, TileMaps &m) {
+  const long long qe[4] = {hd, c.n_heads, c.n_tokens, 1}, qs[4] = {1, c.q_sh, c.q_st, 0};
+  const int qb[4] = {64, c.group, TILE_M / c.group, 1}, kb[4] = {64, tile_box(paged, c.page), 1, 1};
+  const long long ke[4] = {hd, paged ? c.page : c.n_tokens, c.n_kv, paged ? c.n_pages : 1};
+  auto keys = [&](CUtensorMap *out, const uint16_t *base, const long long *st) {
+    const long long str[4] = {1, paged ? st[2] : st[0], st[1], paged ? st[0] : 0};
+    return tensor_map(fn, out, base, f16, 4, ke, str, kb);
+  };
+  return tensor_map(fn, &m.q, c.q, f16, 4, qe, qs, qb) && keys(&m.k, c.k, c.k_st) && keys(&m.v, c.v, c.v_st);
 }
 
 template <int HD, bool F16, bool PAGED>

@@ -231,7 +231,7 @@ __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendCall c)
 constexpr int MAX_DEV = 64;
 struct DevInfo {
   int sms = 0;
-  TileEncodeFn encode = nullptr;           // cuTensorMapEncodeTiled
+  TensorMapFn encode = nullptr;            // cuTensorMapEncodeTiled
   cudaError_t err = cudaSuccess;
 };
 
@@ -256,7 +256,7 @@ int device_info(const DevInfo **out) {
       void *p = nullptr;
       cudaDriverEntryPointQueryResult q;
       d.err = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q);
-      if (q == cudaDriverEntryPointSuccess) d.encode = reinterpret_cast<TileEncodeFn>(p);
+      if (q == cudaDriverEntryPointSuccess) d.encode = reinterpret_cast<TensorMapFn>(p);
     }
   });
   if (d.err != cudaSuccess) return qtb_fail(QTB_E_CUDA, "paged operators on device %d: %s", dev, cudaGetErrorString(d.err));
@@ -268,6 +268,12 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 bool rows16(const int64_t *st, int n, int elem) {
   for (int i = 0; i < n; i++)
     if (st[i] < 0 || st[i] * elem % 16) return false;
+  return true;
+}
+// Strides that a tensor map can hold: an expanded axis (stride 0) it cannot.
+bool spread(const int64_t *st, const int64_t *ext, int n) {
+  for (int i = 0; i < n; i++)
+    if (ext[i] > 1 && (st[i] <= 0 || st[i] >= (1ll << 39))) return false;
   return true;
 }
 
@@ -293,10 +299,16 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
     return qtb_fail(QTB_E_INVALID, "strides must be non-negative multiples of 16 bytes");
   if (paged) {
     if (d->page < 16 || d->page % 16 || d->page > 65536) return qtb_fail(QTB_E_INVALID, "page %lld: a multiple of 16", (long long)d->page);
-    if (d->n_pages < 0 || d->n_pages > INT_MAX || d->table_cols < 0 || d->table_cols > (1 << 30) || d->table_cols * d->page > (1 << 30) || d->table_stride < 0)
+    if (d->n_pages < 1 || d->n_pages >= INT_MAX || d->table_cols < 0 || d->table_cols > (1 << 30) || d->table_cols * d->page > (1 << 30) || d->table_stride < 0)
       return qtb_fail(QTB_E_INVALID, "%lld pages, %lld table columns", (long long)d->n_pages, (long long)d->table_cols);
     if ((d->n_req && !d->kv_len) || (d->n_req && d->table_cols && !d->table) || (d->n_pages && (!d->k || !d->v)))
       return qtb_fail(QTB_E_INVALID, "null pointer");
+  }
+  {
+    const int64_t qx[2] = {d->n_tokens, d->n_heads}, px[3] = {d->n_pages, d->n_kv, d->page}, tx[2] = {d->n_tokens, d->n_kv};
+    if (!spread(d->q_stride, qx, 2) || !spread(d->out_stride, qx, 2) || !spread(d->k_stride, paged ? px : tx, paged ? 3 : 2) ||
+        !spread(d->v_stride, paged ? px : tx, paged ? 3 : 2))
+      return qtb_fail(QTB_E_INVALID, "an axis of q, k, v or out is expanded (stride 0)");
   }
   c = AttnCall{};
   c.q = static_cast<const uint16_t *>(d->q); c.k = static_cast<const uint16_t *>(d->k); c.v = static_cast<const uint16_t *>(d->v);
@@ -324,7 +336,7 @@ struct AttnPlan {
 };
 AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged) {
   AttnPlan p;
-  p.tiles = tile_form(c, paged);
+  p.tiles = tile_form(c);
   p.limit = !p.tiles ? INT_MAX : paged ? ROWS_M : 0;
   if (p.tiles && paged && d->max_new > 0 && d->max_new * c.group <= ROWS_M) {
     p.tiles = false;
@@ -348,11 +360,12 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == QTB_T_F16;
   const int hd = (int)d->head_dim;
-  TileMaps maps;
-  if (p.tiles && !tile_maps(c, paged, f16, hd, dev->encode, maps))
+  TileMaps tm;
+  RowsMaps rm;
+  if ((p.tiles && !tile_maps(c, paged, f16, hd, dev->encode, tm)) || (p.rows && !rows_maps(c, paged, f16, hd, dev->encode, rm)))
     return qtb_fail(QTB_E_UNSUPPORTED, "q, k or v have strides or extents that a tensor map cannot hold");
-  if (p.rows) PAGED_TRY(rows_launch(c, paged, f16, hd, dev->sms, p.limit, d->workspace, st));
-  if (p.tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, maps, dev->sms, p.limit, st));
+  if (p.rows) PAGED_TRY(rows_launch(c, paged, f16, hd, rm, dev->sms, p.limit, d->workspace, st));
+  if (p.tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, tm, dev->sms, p.limit, st));
   return QTB_OK;
 }
 

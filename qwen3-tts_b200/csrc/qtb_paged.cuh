@@ -4,6 +4,7 @@
 #pragma once
 #include "qtb_device.cuh"
 #include "../../include/qwen3tts_b200.h"
+#include <cuda.h>
 
 namespace qtb {
 
@@ -73,19 +74,52 @@ QTB_DEV void ldsm_x4(uint32_t (&r)[4], const void *row_addr) {
                : "r"(smem_u32(row_addr))
                : "memory");
 }
-// 16 bytes global -> shared, or 16 zero bytes when !ok (nothing is read then).
-QTB_DEV void cp16_zfill(void *dst, const void *src, bool ok) {
-  asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0)
-               : "memory");
+// Tiled TMA loads of a 4- or 5-dimensional box (no multicast).
+QTB_DEV void tma_load_4d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      : "memory");
 }
-QTB_DEV void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-QTB_DEV void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+QTB_DEV void tma_load_5d(void *dst, const CUtensorMap *map, int x, int y, int z, int w, int v, uint64_t *bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+          smem_u32(dst)),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(v), "r"(smem_u32(bar))
+      : "memory");
+}
+QTB_DEV void mbar_arrive(uint64_t *bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 // A launch marked programmatic may start while its predecessor still runs:
 // pdl_wait returns when that one's writes are visible, pdl_release lets the
 // successor start.
 QTB_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 QTB_DEV void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// ------------------------------------------------------------------ host ---
+typedef CUresult (*TensorMapFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The map of a tensor of two-byte values (extents and strides innermost first,
+// the innermost stride 1) in boxes with the 128-byte swizzle; what lies outside
+// reads as zeros.
+static inline bool tensor_map(TensorMapFn fn, CUtensorMap *out, const void *base, bool f16, int rank, const long long *ext,
+                              const long long *stride, const int *box) {
+  cuuint64_t dims[5], bytes[4];
+  cuuint32_t b[5], one[5];
+  for (int i = 0; i < rank; i++) {
+    dims[i] = (cuuint64_t)ext[i];
+    b[i] = (cuuint32_t)box[i];
+    one[i] = 1;
+    if (i) bytes[i - 1] = ext[i] > 1 ? (cuuint64_t)stride[i] * 2 : 128;   // of an axis of one, any will do
+  }
+  return fn && fn(out, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (cuuint32_t)rank, const_cast<void *>(base),
+                  dims, bytes, b, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 }  // namespace qtb

@@ -47,7 +47,7 @@ _this_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream   # what torch.cuda.current_stream(i).cuda_stream is, without the object
 
 _calls = None
-_workspace = {}              # bytes by (device, head_dim, form)
+_workspace = {}              # bytes by (device, head_dim, paged?, positive scale?)
 
 
 def _lib():
@@ -191,15 +191,14 @@ def _attend(q, k, v, cu, kv_len, table, pool, max_new, max_kv, scale, causal, wi
             0 if status is None else _index("status", status, dev, 1))
     tail = (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2] if pool else 0, vs[0], vs[1], vs[2] if pool else 0,
             width, cols, page, pages, n, t, h, kv, d, max_new, max_kv, _TYPES[kind], causal, window or 0, scale)
-    # the workspace of ordinary calls depends on device, head_dim and form alone
-    key = (dev, d, pool) if scale > 0 and 0 not in ks and 0 not in vs and 0 not in qs else None
+    key = (dev, d, pool, scale > 0)          # what the workspace's size depends on
     size = _workspace.get(key)
     if size is None:
         with torch.cuda.device(dev):
             size = L.qtb_attn_workspace(_ATTN(*head, 0, 0, *tail), pool)
         if size < 0:
             Q.check(size)
-        if key:
+        if n and t:
             _workspace[key] = size
     at, ws = 0, None
     if size:
