@@ -10,8 +10,8 @@
 // 64-key chunk) units of the whole call are dealt out to the grid in equal
 // runs, whatever the requests' lengths.  An item that a block holds whole is
 // written at once; one that is cut leaves its parts (O, m, l in f32) in the
-// workspace, and rows_join_kernel adds them in block order, so results do not
-// depend on timing.
+// workspace, and join_kernel adds them in block order, so results do not depend
+// on timing.
 //
 // m is renewed lazily, when a score passes it by 2^8: until then the
 // probabilities are at most 2^8 and the quotient O / l does not care.
@@ -28,15 +28,8 @@
 namespace qtb {
 
 constexpr int ROWS_WARPS = 4, ROWS_THREADS = 32 * (ROWS_WARPS + 1), ROWS_M = 16, ROWS_CHUNK = 64, ROWS_PER_SM = 2;
-constexpr int ROWS_JOIN_WARPS = 8;
 constexpr long long ROWS_WAIT = 4000000000ll;   // cycles: about two seconds
 
-// Where a cut item's parts are, per block: the request, row group and head of
-// the item that the block starts and does not finish, and the last block that
-// holds a part of it (-1: none).
-struct RowsCut {
-  int r, rg, h, last;
-};
 struct RowsMaps {
   CUtensorMap k, v;
 };
@@ -90,7 +83,7 @@ struct RowsShared {
 template <int HD, bool F16, bool PAGED>
 __global__ void __launch_bounds__(ROWS_THREADS, ROWS_PER_SM)
 rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_limit, int box, float *__restrict__ parts,
-            RowsCut *__restrict__ cuts) {
+            AttnCut *__restrict__ cuts) {
   constexpr int KS = HD / 16;              // k-steps of Q K^T
   constexpr int NT = HD / 8;               // 8-wide output tiles
   constexpr int STAGES = rows_stages<HD>(), KEYS_B = rows_keys_bytes<HD>();
@@ -401,7 +394,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
             const long long end = u0 + u + (cur.chunks - 1 - cur.ch);
             int b = (int)((end * blocks) / total);
             while (b + 1 < blocks && total * (b + 1) / blocks <= end) b++;
-            cuts[blockIdx.x] = RowsCut{cur.r, cur.rg, cur.h, b};
+            cuts[blockIdx.x] = AttnCut{b, cur.a.t0, cur.a.n, cur.h * c.group, cur.rg * ROWS_M, ROWS_M, {0, 0}};
           }
         }
       }
@@ -412,62 +405,10 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
   }
 }
 
-// Joins the parts of the item that block blockIdx.x cut: part 1 of that block,
-// then part 0 of the following ones, in that order.  A warp has a row, a lane
-// HD / 32 of its dims.
-template <int HD, bool F16, bool PAGED>
-__global__ void __launch_bounds__(32 * ROWS_JOIN_WARPS)
-rows_join_kernel(const AttnCall c, const float *__restrict__ parts, const RowsCut *__restrict__ cuts) {
-  constexpr int PF = rows_part_floats<HD>(), V = HD / 32, UNROLL = 8;
-  pdl_wait();
-  const RowsCut cut = cuts[blockIdx.x];
-  if (cut.last < 0) return;
-  const AttnReq a = attn_request<PAGED>(c, cut.r);
-  const int lane = threadIdx.x & 31, b0 = blockIdx.x, n = cut.last - b0 + 1;
-  auto part = [&](int i) { return parts + (long long)(2 * (b0 + i) + (i == 0 ? 1 : 0)) * PF; };
-  for (int row = threadIdx.x >> 5; row < ROWS_M; row += ROWS_JOIN_WARPS) {
-    const int rr = cut.rg * ROWS_M + row, t = rr / c.group, h = cut.h * c.group + rr - t * c.group;
-    if (t >= a.n) return;
-    float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, part(i)[ROWS_M * HD + 2 * row]);
-    m = warp_max(m);
-    const float base = m == -INFINITY ? 0.f : m;
-    float l = 0.f, o[V] = {};
-    for (int i0 = 0; i0 < n; i0 += UNROLL) {
-      float x[UNROLL][V], f[UNROLL], z[UNROLL];
-#pragma unroll
-      for (int i = 0; i < UNROLL; i++) {
-        const float *p = part(min(i0 + i, n - 1));
-#pragma unroll
-        for (int v = 0; v < V; v += 2) {
-          const float2 y = *reinterpret_cast<const float2 *>(p + row * HD + V * lane + v);
-          x[i][v] = y.x; x[i][v + 1] = y.y;
-        }
-        f[i] = p[ROWS_M * HD + 2 * row];
-        z[i] = p[ROWS_M * HD + 2 * row + 1];
-      }
-#pragma unroll
-      for (int i = 0; i < UNROLL; i++) {
-        if (i0 + i >= n) break;
-        const float w = exp2_approx(f[i] - base);
-        l += z[i] * w;
-#pragma unroll
-        for (int v = 0; v < V; v++) o[v] += x[i][v] * w;
-      }
-    }
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    const long long at = a.t0 + t;
-    uint16_t *op = c.out + at * c.o_st + h * c.o_sh + V * lane;
-#pragma unroll
-    for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t *>(op + v) = pack2<F16>(o[v] * inv, o[v + 1] * inv);
-    if (c.lse && lane == 0) c.lse[at * c.n_heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-  }
-}
-
 // ------------------------------------------------------------------ host ---
 static inline size_t rows_workspace(int hd, int sms) {
   const size_t grid = (size_t)sms * ROWS_PER_SM;
-  return grid * 16 + grid * 2 * (size_t)(hd == 128 ? rows_part_floats<128>() : rows_part_floats<64>()) * 4;
+  return grid * sizeof(AttnCut) + grid * 2 * (size_t)(hd == 128 ? rows_part_floats<128>() : rows_part_floats<64>()) * 4;
 }
 
 // Keys in boxes of a run of a page's positions, all dims: [dim / 64][position][64].
@@ -488,48 +429,41 @@ static inline bool rows_maps(const AttnCall &c, bool paged, bool f16, int hd, Te
 }
 
 template <int HD, bool F16, bool PAGED>
-static cudaError_t rows_run(bool prepare, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, void *ws, cudaStream_t st) {
+static cudaError_t rows_run(bool prepare, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, int max_rows, void *ws,
+                            cudaStream_t st) {
   if (prepare)
     return cudaFuncSetAttribute(rows_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem<HD>());
   const int grid = sms * ROWS_PER_SM;
-  RowsCut *cuts = static_cast<RowsCut *>(ws);
-  float *parts = reinterpret_cast<float *>(static_cast<char *>(ws) + (size_t)grid * sizeof(RowsCut));
+  AttnCut *cuts = static_cast<AttnCut *>(ws);
+  float *parts = reinterpret_cast<float *>(cuts + grid);
   rows_kernel<HD, F16, PAGED><<<grid, ROWS_THREADS, rows_smem<HD>(), st>>>(*c, *m, row_limit, rows_box(PAGED, c->page), parts, cuts);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[1];
-  cfg.gridDim = dim3(grid);
-  cfg.blockDim = dim3(32 * ROWS_JOIN_WARPS);
-  cfg.stream = st;
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, rows_join_kernel<HD, F16, PAGED>, *c, (const float *)parts, (const RowsCut *)cuts);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  return launch_early(join_kernel<HD, F16, ROWS_M, 1, JOIN_WARPS>, dim3(grid, max_rows), 32 * JOIN_WARPS, 0, st, *c, (const float *)parts,
+                      (const AttnCut *)cuts);
 }
-// Requests with at most row_limit query rows to a key head are served.
-static inline cudaError_t rows_any(bool prepare, int which, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, void *ws,
-                                   cudaStream_t st) {
+// Requests with at most row_limit query rows to a key head are served; max_rows
+// is how many rows (of 16) an item may have, as far as known.
+static inline cudaError_t rows_any(bool prepare, int which, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, int max_rows,
+                                   void *ws, cudaStream_t st) {
   switch (which) {
-    case 0: return rows_run<64, false, false>(prepare, c, m, sms, row_limit, ws, st);
-    case 1: return rows_run<64, false, true>(prepare, c, m, sms, row_limit, ws, st);
-    case 2: return rows_run<64, true, false>(prepare, c, m, sms, row_limit, ws, st);
-    case 3: return rows_run<64, true, true>(prepare, c, m, sms, row_limit, ws, st);
-    case 4: return rows_run<128, false, false>(prepare, c, m, sms, row_limit, ws, st);
-    case 5: return rows_run<128, false, true>(prepare, c, m, sms, row_limit, ws, st);
-    case 6: return rows_run<128, true, false>(prepare, c, m, sms, row_limit, ws, st);
-    default: return rows_run<128, true, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 0: return rows_run<64, false, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 1: return rows_run<64, false, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 2: return rows_run<64, true, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 3: return rows_run<64, true, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 4: return rows_run<128, false, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 5: return rows_run<128, false, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 6: return rows_run<128, true, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    default: return rows_run<128, true, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
   }
 }
 static inline cudaError_t rows_prepare() {
   for (int i = 0; i < 8; i++)
-    if (cudaError_t e = rows_any(true, i, nullptr, nullptr, 0, 0, nullptr, nullptr)) return e;
+    if (cudaError_t e = rows_any(true, i, nullptr, nullptr, 0, 0, 0, nullptr, nullptr)) return e;
   return cudaSuccess;
 }
 static inline cudaError_t rows_launch(const AttnCall &c, bool paged, bool f16, int hd, const RowsMaps &m, int sms, int row_limit,
-                                      void *ws, cudaStream_t st) {
-  return rows_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, row_limit, ws, st);
+                                      int max_rows, void *ws, cudaStream_t st) {
+  return rows_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, row_limit, max_rows, ws, st);
 }
 
 }  // namespace qtb

@@ -25,6 +25,14 @@
 // The probabilities of a tile start from the old maximum at once, beside the new
 // maximum's search, and are thrown away in the rare tile that outgrows it.
 //
+// An item of work is a tile pair and a key head.  Where there are many to a
+// block, they are dealt out whole, longest first.  Where there are few, the key
+// tiles of all are dealt out in equal runs, whatever the requests' lengths; an
+// item that is cut between blocks leaves its parts in the workspace, and
+// join_kernel adds them.  (Runs of many items would also walk the keys at as
+// many places at once as there are blocks: a prompt of 16384 tokens, 16 / 8
+// heads, took 993 us so, and 827 us with whole items.)
+//
 // Products are issued in order, so the commit that completes S of tile j also
 // says that P V of tile j - 1 is in O: the softmax warps may scale O then.
 // Every wait is bounded; one that runs out raises QTB_PS_TIMEOUT and all roles
@@ -39,6 +47,8 @@ constexpr int TILE_THREADS = 384, TILE_M = 128, TILE_N = 128;
 // (64512 in all); the softmax warps, a row of S each, take what the loading and
 // issuing warpgroup gives up: 256 * 200 + 128 * 96 = 63488.
 constexpr int TILE_REGS_SOFTMAX = 200, TILE_REGS_OTHER = 96;
+constexpr int TILE_DEAL = 4;               // items to a block from which on they are dealt out whole
+constexpr int TILE_CUT = 2;                // key tiles that a block has of an item at least, where it has not all
 constexpr int TILE_SEGS = 128;             // runs of requests that the in-block search tells apart
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
@@ -48,6 +58,9 @@ template <int HD>
 constexpr int tile_kv_bytes() { return TILE_N * HD * 2; }
 template <int HD>
 constexpr int tile_operands() { return 2 * TILE_M * HD * 2 + tile_stages<HD>() * tile_kv_bytes<HD>(); }
+
+template <int HD>
+constexpr int tile_part_floats() { return TILE_M * (HD + 2); }   // O rows, then (m, l) pairs
 
 struct TileMaps {
   CUtensorMap q, k, v;
@@ -66,6 +79,9 @@ struct TileShared {
   TileSync sy;
   int pre[TILE_SEGS + 1];                  // query tile pairs before each run of requests
   int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS];   // the requests themselves, where a run is one
+  long long scan[TILE_THREADS / 32];
+  int item[2], off[2];                     // the block's first item and place in it, and where the next block's are
+  long long base;                          // units of work before item[1]
 };
 template <int HD>
 constexpr int tile_smem() { return tile_operands<HD>() + (int)sizeof(TileShared); }
@@ -101,6 +117,13 @@ QTB_DEV void tmem_ld8_async(uint32_t taddr, float *r) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
       : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7])
+      : "r"(taddr));
+}
+QTB_DEV void tmem_ld16_async(uint32_t taddr, float *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]),
+        "=f"(r[8]), "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15])
       : "r"(taddr));
 }
 QTB_DEV void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
@@ -174,13 +197,15 @@ struct TileItem {
   int low;              // keys before this are seen by no row of the pair
   int k0;               // first key of key tile 0 (a multiple of 128)
   int tok0, tok1;       // tokens in each tile
-  int n0, n1;           // key tiles of each
+  int from, n0, n1;     // key tiles [from, n0) are this block's for query tile 0, [from, n1) for tile 1
+  bool whole;           // those are all
   int high;             // keys at and past this are seen by no row
 };
 
 template <int HD, bool F16, bool PAGED>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
-tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int tpt, int box) {
+tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int tpt, int box,
+            float *__restrict__ parts, AttnCut *__restrict__ cuts) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
   extern __shared__ __align__(1024) unsigned char tile_smem_base[];
@@ -241,17 +266,10 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = sy.tmem;
-  const int items = pairs * c.n_kv;        // the host has bounded it
 
-  // This block's n-th item.  Items go longest causal tiles first (pairs from the
-  // last to the first, key heads inside) and are dealt to the blocks to and fro,
-  // so that the sums come out alike.  False past the end.
-  auto get_item = [&](int n, TileItem &it) {
-    const unsigned i = (unsigned)n * gridDim.x + (n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (i >= (unsigned)items) return false;
-    int p = (int)(i / (unsigned)c.n_kv);
-    it.h = (int)i - p * c.n_kv;
-    p = pairs - 1 - p;
+  // A query tile pair of a request and its keys; the items of the call are
+  // (pair, key head), numbered pair by pair.
+  auto get_pair = [&](int p, TileItem &it) {
     int lo = 0;                            // the last run that starts at or before p
 #pragma unroll 1
     for (int step = TILE_SEGS / 2; step; step >>= 1)
@@ -278,6 +296,109 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     it.n0 = hi0 > it.low ? (hi0 - it.k0 + TILE_N - 1) / TILE_N : 0;
     it.n1 = it.tok1 > 0 && hi1 > it.low ? (hi1 - it.k0 + TILE_N - 1) / TILE_N : 0;
     it.high = max(hi0, hi1);
+  };
+  // --- this block's run of work.  An item costs its key tiles and one for getting
+  // started; boundaries between blocks move to an item's start or end where less
+  // than TILE_CUT key tiles would be left on that side.
+  const int items = pairs * c.n_kv;        // the host has bounded it
+  const bool deal = !parts || items >= TILE_DEAL * (int)gridDim.x;
+  if (deal) {
+    if (tid == 0 && parts) cuts[blockIdx.x].last = -1;
+  } else {
+    auto cost_of = [&](int p) {
+      TileItem it;
+      get_pair(p, it);
+      return max(it.n0, it.n1) + 1;
+    };
+    auto scan = [&](long long v, long long &total) {      // inclusive, over the block
+      long long x = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) sh.scan[warp] = x;
+      __syncthreads();
+      total = 0;
+#pragma unroll
+      for (int w = 0; w < TILE_THREADS / 32; w++) {
+        if (w < warp) x += sh.scan[w];
+        total += sh.scan[w];
+      }
+      return x;
+    };
+    int cost = tid < pairs ? cost_of(tid) : 0;
+    long long total, upto = scan(cost, total);
+    for (int p0 = TILE_THREADS; p0 < pairs; p0 += TILE_THREADS) {
+      long long more;
+      scan(p0 + tid < pairs ? cost_of(p0 + tid) : 0, more);
+      total += more;
+    }
+    total *= c.n_kv;
+    const long long blocks = max(min((long long)gridDim.x, total / (2 * TILE_CUT)), 1ll);
+    if (tid < 2) {                         // where no boundary is found: past the end
+      sh.item[tid] = items;
+      sh.off[tid] = 0;
+    }
+    long long before = 0;
+    for (int p0 = 0; p0 < pairs; p0 += TILE_THREADS) {
+      long long all;
+      if (p0 > 0) cost = p0 + tid < pairs ? cost_of(p0 + tid) : 0;
+      if (pairs > TILE_THREADS) upto = scan(cost, all);
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        if (blockIdx.x + e >= blocks) continue;
+        const long long x = total * (blockIdx.x + e) / blocks, first = (before + upto - cost) * c.n_kv;
+        if (x < first || x >= first + (long long)cost * c.n_kv) continue;
+        int h = (int)((unsigned)(x - first) / (unsigned)cost), off = (int)(x - first) - h * cost;
+        if (off < 1 + TILE_CUT) off = 0;
+        else if (cost - off < TILE_CUT) { off = 0; h++; }
+        sh.item[e] = (p0 + tid) * c.n_kv + h;   // h may be n_kv: the next pair's first
+        sh.off[e] = off;
+        if (e) sh.base = first + (long long)h * cost;
+      }
+      if (pairs > TILE_THREADS) before += all;
+    }
+    __syncthreads();
+    if (tid == 10 * 32) {                  // an item that this block begins and does not finish
+      int last = -1;
+      TileItem it;
+      if (blockIdx.x < blocks && sh.off[1] > 0 && !(sh.item[0] == sh.item[1] && sh.off[0] > 0)) {
+        get_pair(sh.item[1] / c.n_kv, it);
+        const int cost = max(it.n0, it.n1) + 1;
+        last = blockIdx.x + 1;
+        for (long long x; last + 1 < blocks && (x = total * (last + 1) / blocks - sh.base) < cost && cost - x >= TILE_CUT;) last++;
+      }
+      cuts[blockIdx.x] = last < 0 ? AttnCut{-1, 0, 0, 0, 0, 0, {0, 0}}
+                                  : AttnCut{last, it.t0, it.end - it.first, (sh.item[1] % c.n_kv) * c.group, it.tok * c.group, tpt * c.group, {0, 0}};
+    }
+  }
+
+  // The block's n-th item and its share of the key tiles: [from, n0) for query
+  // tile 0, [from, n1) for tile 1.  False past the end.  Whole items go from the
+  // last pair to the first (longest causal ones first), key heads inside, and to
+  // and fro over the blocks, so that the sums come out alike.
+  auto get_item = [&](int n, TileItem &it) {
+    int i, from = 0, off1 = 0;
+    if (deal) {
+      i = n * (int)gridDim.x + (int)(n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      if (i >= items) return false;
+    } else {
+      i = sh.item[0] + n;
+      if (n == 0) from = max(sh.off[0] - 1, 0);
+      if (i >= sh.item[1]) off1 = sh.off[1];
+      if (i > sh.item[1] || (i == sh.item[1] && off1 == 0)) return false;
+    }
+    const int p = (int)((unsigned)i / (unsigned)c.n_kv);
+    get_pair(deal ? pairs - 1 - p : p, it);
+    it.h = i - p * c.n_kv;
+    const int all = max(it.n0, it.n1), to = off1 > 0 ? off1 - 1 : all;
+    it.from = from;
+    it.whole = from == 0 && to == all;
+    it.n0 = max(min(to, it.n0), from);
+    it.n1 = max(min(to, it.n1), from);
     return true;
   };
   // Bounded wait of a whole warp; false: this or another role gave up.
@@ -307,8 +428,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int tiles = max(it.n0, it.n1);
-      if (tiles == 0) continue;
+      const int to = max(it.n0, it.n1);
+      if (to == it.from) continue;
       auto load_q = [&]() {
         if (!wait(&sy.q_empty, (n_items & 1) ^ 1)) return false;
         if (lane == 0) {
@@ -321,7 +442,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         n_items++;
         return true;
       };
-      for (int j = 0; j < tiles && ok; j++) {
+      for (int j = it.from; j < to && ok; j++) {
         const int kb = it.k0 + j * TILE_N;
         // this lane's box of the key tile: positions [pos, pos + box), 64 dims
         const int boxes = PAGED ? TILE_N / box : 1, bi = lane / (HD / 64), x = lane % (HD / 64);
@@ -349,7 +470,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
           }
           fill++;
           // the queries' buffer may still serve the item before: its keys go first
-          if (kv == 0 && j == 0 && !load_q()) { ok = false; break; }
+          if (kv == 0 && j == it.from && !load_q()) { ok = false; break; }
         }
       }
     }
@@ -371,8 +492,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int tiles = max(it.n0, it.n1);
-      if (tiles == 0) continue;
+      const int to = max(it.n0, it.n1);
+      if (to == it.from) continue;
       if (!wait(&sy.q_full, n_items & 1)) break;
       n_items++;
       auto scores = [&](int t, int st) {
@@ -391,17 +512,17 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       int st = (int)(fill % STAGES);
       if (!(ok = wait(&sy.kv_full[st], (fill / STAGES) & 1))) break;
       issued = true;
-      if (it.n0 > 0) scores(0, st);
-      if (it.n1 > 0) scores(1, st);
+      if (it.n0 > it.from) scores(0, st);
+      if (it.n1 > it.from) scores(1, st);
       if (elect_one()) {
         umma_commit(&sy.kv_empty[st]);
-        if (tiles == 1) umma_commit(&sy.q_empty);
+        if (to == it.from + 1) umma_commit(&sy.q_empty);
       }
       __syncwarp();
       fill++;
-      for (int j = 0; j < tiles && ok; j++) {
+      for (int j = it.from; j < to && ok; j++) {
         const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
-        const bool more = j + 1 < tiles;
+        const bool more = j + 1 < to;
 #pragma unroll
         for (int t = 0; t < 2; t++) {
           const int n = t ? it.n1 : it.n0;
@@ -412,14 +533,14 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
           uint32_t par = (p_n >> t) & 1;
           if (lane == 1) { bar = &sy.kv_full[sv]; par = (fill / STAGES) & 1; }
           if (lane == 2 && more) { bar = &sy.kv_full[sk]; par = ((fill + 1) / STAGES) & 1; }
-          if (lane == 3 && j == 0) { bar = &sy.o_empty[t]; par = ((o_n >> t) & 1) ^ 1; }
+          if (lane == 3 && j == it.from) { bar = &sy.o_empty[t]; par = ((o_n >> t) & 1) ^ 1; }
           if (!(ok = wait(bar, par))) break;
           tc_fence_after();
           const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
           const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
           if (elect_one()) {
 #pragma unroll
-            for (int ks = 0; ks < TILE_N / 32; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, (j | ks) != 0);
+            for (int ks = 0; ks < TILE_N / 32; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, j > it.from || ks > 0);
           }
           __syncwarp();
           if (!(ok = wait(&sy.p_full[t][1], (p_n >> t) & 1))) break;
@@ -438,7 +559,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         if (elect_one()) {
           umma_commit(&sy.kv_empty[sv]);
           if (more) umma_commit(&sy.kv_empty[sk]);
-          if (j + 2 == tiles) umma_commit(&sy.q_empty);
+          if (j + 2 == to) umma_commit(&sy.q_empty);
         }
         __syncwarp();
         fill += more ? 2 : 1;
@@ -460,7 +581,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int i = 0;; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int tiles = max(it.n0, it.n1), n = t ? it.n1 : it.n0, n_tok = t ? it.tok1 : it.tok0;
+      const int to = max(it.n0, it.n1), n = t ? it.n1 : it.n0, n_tok = t ? it.tok1 : it.tok0;
       const int tt = row / c.group;
       const int pos = it.first + it.tok + t * tpt + tt;           // this row's position
       const int tk = tt < n_tok ? it.t0 + it.tok + t * tpt + tt : -1;   // its packed token (-1: no row)
@@ -472,7 +593,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
-      for (int j = 0; j < n; j++) {
+      for (int j = it.from; j < n; j++) {
         if (!(ok = wait(&sy.s_full[t], s_n & 1))) break;
         s_n++;
         tc_fence_after();
@@ -495,7 +616,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
           }
           if (kb < it.low || kb + TILE_N > it.high) {
             // keys that no row sees: their V may be anything, and 0 * NaN is NaN
-            const uint32_t f = fill + 2 * j + 1;
+            const uint32_t f = fill + 2 * (j - it.from) + 1;
             unsigned char *v = s_kv + (f % STAGES) * KV_B;
             if (!(ok = wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1))) break;
             if (kb + row < it.low || kb + row >= it.high) {
@@ -547,7 +668,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         // Past the first tile m rarely moves: the probabilities start from the old
         // one while the maximum is taken beside them, and are made anew where a row
         // has outgrown it.
-        bool anew = j == 0;
+        bool anew = j == it.from;
         if (!anew) {
           sum[0] = sum[1] = 0;
 #pragma unroll
@@ -560,7 +681,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
             const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_approx(m - m2);
             m = m2;
             l *= f;
-            if (j > 0) {
+            if (j > it.from) {
 #pragma unroll 1
               for (int x = 0; x < HD / 8; x++) {
                 float o[8];
@@ -586,33 +707,17 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         l += la + lb;
       }
       if (!ok) break;
-      fill += 2 * tiles;
-      if (n > 0) {
+      fill += 2 * (to - it.from);
+      const bool some = n > it.from;
+      if (some) {
         if (!wait(&sy.o_full[t], o_n & 1)) break;
         o_n++;
         tc_fence_after();
       }
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
       // A thread has a row, so that its 16-byte stores would each touch a line of
       // their own: four neighbours turn their 4 x 4 units first, and a store
       // instruction writes 64 bytes of each of 8 rows.
-      const long long at = tk >= 0 ? (long long)tk * c.o_st + head * c.o_sh : -1;
-      long long rows[4];
-#pragma unroll
-      for (int y = 0; y < 4; y++) rows[y] = __shfl_sync(0xffffffffu, at, (lane & ~3) + y);
-#pragma unroll 1
-      for (int x = 0; x < HD / 32; x++) {
-        float o[32];
-        if (n > 0) {
-          tmem_ld32_async(o_at + 32 * x, o);
-          tmem_ld_wait();
-        }
-        uint32_t w[4][4];
-#pragma unroll
-        for (int y = 0; y < 4; y++)
-#pragma unroll
-          for (int z = 0; z < 4; z++)
-            w[y][z] = n > 0 ? pack2<F16>(o[8 * y + 2 * z] * inv, o[8 * y + 2 * z + 1] * inv) : 0u;
+      auto turn = [&](uint32_t (&w)[4][4]) {
 #pragma unroll
         for (int bit = 1; bit <= 2; bit <<= 1)
 #pragma unroll
@@ -625,18 +730,56 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
               else w[y | bit][z] = got;
             }
           }
+      };
+      if (it.whole) {
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
+        const long long at = tk >= 0 ? (long long)tk * c.o_st + head * c.o_sh : -1;
+        long long rows[4];
 #pragma unroll
-        for (int y = 0; y < 4; y++)
-          if (rows[y] >= 0)
-            *reinterpret_cast<uint4 *>(c.out + rows[y] + 32 * x + 8 * (lane & 3)) = make_uint4(w[y][0], w[y][1], w[y][2], w[y][3]);
-        __syncwarp();
+        for (int y = 0; y < 4; y++) rows[y] = __shfl_sync(0xffffffffu, at, (lane & ~3) + y);
+#pragma unroll 1
+        for (int x = 0; x < HD / 32; x++) {
+          float o[32];
+          if (some) {
+            tmem_ld32_async(o_at + 32 * x, o);
+            tmem_ld_wait();
+          }
+          uint32_t w[4][4];
+#pragma unroll
+          for (int y = 0; y < 4; y++)
+#pragma unroll
+            for (int z = 0; z < 4; z++)
+              w[y][z] = some ? pack2<F16>(o[8 * y + 2 * z] * inv, o[8 * y + 2 * z + 1] * inv) : 0u;
+          turn(w);
+#pragma unroll
+          for (int y = 0; y < 4; y++)
+            if (rows[y] >= 0)
+              *reinterpret_cast<uint4 *>(c.out + rows[y] + 32 * x + 8 * (lane & 3)) = make_uint4(w[y][0], w[y][1], w[y][2], w[y][3]);
+          __syncwarp();
+        }
+        if (tk >= 0 && c.lse) c.lse[(long long)tk * c.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      } else {
+        float *part = parts + ((long long)(2 * blockIdx.x + (it.from == 0 ? 1 : 0)) * 2 + t) * tile_part_floats<HD>();
+        if (some) {
+#pragma unroll 1
+          for (int x = 0; x < HD / 16; x++) {
+            uint32_t w[4][4];
+            tmem_ld16_async(o_at + 16 * x, reinterpret_cast<float *>(w));
+            tmem_ld_wait();
+            turn(w);
+#pragma unroll
+            for (int y = 0; y < 4; y++)
+              *reinterpret_cast<uint4 *>(part + ((row & ~3) + y) * HD + 16 * x + 4 * (lane & 3)) = make_uint4(w[y][0], w[y][1], w[y][2], w[y][3]);
+            __syncwarp();
+          }
+        }
+        *reinterpret_cast<float2 *>(part + TILE_M * HD + 2 * row) = make_float2(m, l);
       }
-      if (n > 0) {
+      if (some) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sy.o_empty[t]);
       }
-      if (tk >= 0 && c.lse) c.lse[(long long)tk * c.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
     }
   }
   tc_fence_before();
@@ -668,39 +811,50 @@ static inline bool tile_maps(const AttnCall &c, bool paged, bool f16, int hd, Te
   return tensor_map(fn, &m.q, c.q, f16, 4, qe, qs, qb) && keys(&m.k, c.k, c.k_st) && keys(&m.v, c.v, c.v_st);
 }
 
+static inline size_t tile_workspace(int hd, int sms) {
+  return (size_t)sms * (sizeof(AttnCut) + 2 * 2 * (size_t)(hd == 128 ? tile_part_floats<128>() : tile_part_floats<64>()) * 4);
+}
+
 template <int HD, bool F16, bool PAGED>
-static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, int grid, int row_limit, cudaStream_t st) {
+static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, int sms, int row_limit, void *ws, cudaStream_t st) {
   if (prepare)
     return cudaFuncSetAttribute(tile_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<HD>());
-  tile_kernel<HD, F16, PAGED><<<grid, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, TILE_M / c->group, tile_box(PAGED, c->page));
-  return cudaGetLastError();
+  const int tpt = TILE_M / c->group, box = tile_box(PAGED, c->page);
+  if (!ws) {                               // whole items only
+    const long long items = ((c->n_tokens + 2 * tpt - 1) / (2 * tpt) + (c->n_req > 1 ? c->n_req : 0)) * (long long)c->n_kv;   // at most
+    tile_kernel<HD, F16, PAGED><<<(int)(items < sms ? items : sms), TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tpt, box, nullptr, nullptr);
+    return cudaGetLastError();
+  }
+  AttnCut *cuts = static_cast<AttnCut *>(ws);
+  float *parts = reinterpret_cast<float *>(cuts + sms);
+  tile_kernel<HD, F16, PAGED><<<sms, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tpt, box, parts, cuts);
+  if (cudaError_t e = cudaGetLastError()) return e;
+  return launch_early(join_kernel<HD, F16, TILE_M, 2, 1>, dim3(sms, 2 * TILE_M / JOIN_WARPS), 32 * JOIN_WARPS, 0, st, *c,
+                      (const float *)parts, (const AttnCut *)cuts);
 }
-static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int grid, int row_limit,
+static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int sms, int row_limit, void *ws,
                                    cudaStream_t st) {
   switch (which) {
-    case 0: return tile_run<64, false, false>(prepare, c, m, grid, row_limit, st);
-    case 1: return tile_run<64, false, true>(prepare, c, m, grid, row_limit, st);
-    case 2: return tile_run<64, true, false>(prepare, c, m, grid, row_limit, st);
-    case 3: return tile_run<64, true, true>(prepare, c, m, grid, row_limit, st);
-    case 4: return tile_run<128, false, false>(prepare, c, m, grid, row_limit, st);
-    case 5: return tile_run<128, false, true>(prepare, c, m, grid, row_limit, st);
-    case 6: return tile_run<128, true, false>(prepare, c, m, grid, row_limit, st);
-    default: return tile_run<128, true, true>(prepare, c, m, grid, row_limit, st);
+    case 0: return tile_run<64, false, false>(prepare, c, m, sms, row_limit, ws, st);
+    case 1: return tile_run<64, false, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 2: return tile_run<64, true, false>(prepare, c, m, sms, row_limit, ws, st);
+    case 3: return tile_run<64, true, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 4: return tile_run<128, false, false>(prepare, c, m, sms, row_limit, ws, st);
+    case 5: return tile_run<128, false, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 6: return tile_run<128, true, false>(prepare, c, m, sms, row_limit, ws, st);
+    default: return tile_run<128, true, true>(prepare, c, m, sms, row_limit, ws, st);
   }
 }
 static inline cudaError_t tile_prepare() {
   for (int i = 0; i < 8; i++)
-    if (cudaError_t e = tile_any(true, i, nullptr, nullptr, 0, 0, nullptr)) return e;
+    if (cudaError_t e = tile_any(true, i, nullptr, nullptr, 0, 0, nullptr, nullptr)) return e;
   return cudaSuccess;
 }
-// Requests with more than row_limit query rows to a key head are served.
+// Requests with more than row_limit query rows to a key head are served; without
+// a workspace no item is cut.
 static inline cudaError_t tile_launch(const AttnCall &c, bool paged, bool f16, int hd, const TileMaps &m, int sms, int row_limit,
-                                      cudaStream_t st) {
-  const int tpp = 2 * (TILE_M / c.group);
-  const long long pairs = c.n_req == 1 ? (c.n_tokens + tpp - 1) / tpp : c.n_tokens / tpp + c.n_req;   // at most
-  const long long items = pairs * c.n_kv;
-  return tile_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, (int)(items < sms ? items : sms),
-                  row_limit, st);
+                                      void *ws, cudaStream_t st) {
+  return tile_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, row_limit, ws, st);
 }
 
 }  // namespace qtb

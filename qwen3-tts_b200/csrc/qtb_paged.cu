@@ -333,8 +333,10 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
 struct AttnPlan {
   bool rows, tiles;
   int limit;               // rows kernel: requests of at most so many rows
+  bool cut;                // tiles: items may be cut between blocks
+  size_t rows_ws, ws;      // bytes: the rows kernel's workspace, then the tiles'
 };
-AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged) {
+AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged, int sms) {
   AttnPlan p;
   p.tiles = tile_form(c);
   p.limit = !p.tiles ? INT_MAX : paged ? ROWS_M : 0;
@@ -342,7 +344,13 @@ AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged) {
     p.tiles = false;
     p.limit = INT_MAX;
   }
+  // one request, or all alike: none has few rows beside many
+  if (p.tiles && (c.n_req == 1 || d->max_new * c.n_req == d->n_tokens) && c.n_tokens / c.n_req * c.group > ROWS_M) p.limit = 0;
   p.rows = p.limit > 0;
+  // a few key tiles are not worth a second launch
+  p.cut = p.tiles && !(d->max_kv > 0 && d->max_kv <= 4 * TILE_N);
+  p.rows_ws = p.rows ? rows_workspace((int)d->head_dim, sms) : 0;
+  p.ws = p.rows_ws + (p.cut ? tile_workspace((int)d->head_dim, sms) : 0);
   return p;
 }
 
@@ -353,8 +361,8 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   if (!c.n_req || !c.n_tokens) return QTB_OK;
   const DevInfo *dev;
   if ((rc = device_info(&dev))) return rc;
-  const AttnPlan p = attn_plan(c, d, paged);
-  const int64_t need = p.rows ? (int64_t)rows_workspace((int)d->head_dim, dev->sms) : 0;
+  const AttnPlan p = attn_plan(c, d, paged, dev->sms);
+  const int64_t need = (int64_t)p.ws;
   if (d->workspace_bytes < need || (need && !d->workspace) || !aligned16(d->workspace))
     return qtb_fail(QTB_E_INVALID, "workspace of %lld bytes on 16: %lld needed", (long long)d->workspace_bytes, (long long)need);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -364,8 +372,10 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   RowsMaps rm;
   if ((p.tiles && !tile_maps(c, paged, f16, hd, dev->encode, tm)) || (p.rows && !rows_maps(c, paged, f16, hd, dev->encode, rm)))
     return qtb_fail(QTB_E_UNSUPPORTED, "q, k or v have strides or extents that a tensor map cannot hold");
-  if (p.rows) PAGED_TRY(rows_launch(c, paged, f16, hd, rm, dev->sms, p.limit, d->workspace, st));
-  if (p.tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, tm, dev->sms, p.limit, st));
+  char *ws = static_cast<char *>(d->workspace);
+  const int max_rows = d->max_new > 0 && d->max_new * c.group < ROWS_M ? (int)d->max_new * c.group : ROWS_M;
+  if (p.rows) PAGED_TRY(rows_launch(c, paged, f16, hd, rm, dev->sms, p.limit, max_rows, ws, st));
+  if (p.tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, tm, dev->sms, p.limit, p.cut ? ws + p.rows_ws : nullptr, st));
   return QTB_OK;
 }
 
@@ -443,7 +453,7 @@ extern "C" int64_t qtb_attn_workspace(const qtb_attn_t *d, int paged) {
   if (!c.n_req || !c.n_tokens) return 0;
   const DevInfo *dev;
   if (int rc = device_info(&dev)) return rc;
-  return paged || attn_plan(c, d, false).rows ? (int64_t)rows_workspace((int)d->head_dim, dev->sms) : 0;
+  return (int64_t)attn_plan(c, d, paged != 0, dev->sms).ws;
 }
 
 extern "C" int qtb_paged_attention(const qtb_attn_t *d, void *stream) { return attend(d, true, stream); }

@@ -99,7 +99,114 @@ QTB_DEV void mbar_arrive(uint64_t *bar) {
 QTB_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 QTB_DEV void pdl_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// ----------------------------------------------------------------- join ----
+// Work that several blocks share leaves its parts in the workspace: block b has
+// room for two, part 0 of an item that began in an earlier block and part 1 of
+// one that goes on in the next.  A part is, for each of its 1 or 2 tiles of M
+// rows, the outputs O [M][HD] and (m, l) [M][2] in f32.  What block b began and
+// did not finish:
+struct AttnCut {
+  int last;                // the last block with a part of it (-1: nothing was cut)
+  int t0, n;               // the request's first packed token, its tokens
+  int head0, row0;         // first query head; index of row 0 among the request's rows of the key head
+  int per_tile;            // rows in use in a tile
+  int pad[2];
+};
+constexpr int JOIN_WARPS = 8;
+
+// Adds the parts of the item that block blockIdx.x cut: part 1 of that block,
+// then part 0 of the following ones.  WPR warps share a row (they take every
+// WPR-th part and join theirs in warp order), a lane has HD / 32 of its dims.
+template <int HD, bool F16, int M, int TILES, int WPR>
+__global__ void __launch_bounds__(32 * JOIN_WARPS)
+join_kernel(const AttnCall c, const float *__restrict__ parts, const AttnCut *__restrict__ cuts) {
+  constexpr int TF = M * (HD + 2), V = HD / 32, UNROLL = 4, ROWS = JOIN_WARPS / WPR;
+  __shared__ float s_o[WPR > 1 ? JOIN_WARPS : 1][HD];
+  __shared__ float2 s_ml[JOIN_WARPS];
+  pdl_wait();
+  const AttnCut cut = cuts[blockIdx.x];
+  if (cut.last < 0) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b0 = blockIdx.x, n = cut.last - b0 + 1, sub = warp % WPR;
+  for (int r0 = blockIdx.y * ROWS; r0 < M * TILES; r0 += gridDim.y * ROWS) {
+    const int row = r0 + warp / WPR, tile = row / M, rr = row - tile * M;
+    const int at = cut.row0 + tile * cut.per_tile + rr, tok = at / c.group, head = cut.head0 + at - tok * c.group;
+    const bool live = rr < cut.per_tile && tok < cut.n;
+    if (WPR > 1 && !live) return;          // the whole block's row
+    float m = -INFINITY, l = 0.f, o[V] = {};
+    if (live) {
+      auto part = [&](int i) { return parts + ((long long)(2 * (b0 + i) + (i == 0 ? 1 : 0)) * TILES + tile) * TF; };
+      for (int i0 = sub; i0 < n; i0 += WPR * UNROLL) {
+        float x[UNROLL][V];
+        float2 ml[UNROLL];
+#pragma unroll
+        for (int i = 0; i < UNROLL; i++) {
+          const float *p = part(min(i0 + i * WPR, n - 1));
+          ml[i] = *reinterpret_cast<const float2 *>(p + M * HD + 2 * rr);
+#pragma unroll
+          for (int v = 0; v < V; v += 2) {
+            const float2 y = *reinterpret_cast<const float2 *>(p + rr * HD + V * lane + v);
+            x[i][v] = y.x; x[i][v + 1] = y.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < UNROLL; i++) {
+          // a part without a visible key has m = -inf, and O that was never written
+          if (i0 + i * WPR >= n || ml[i].x == -INFINITY) continue;
+          const float m2 = fmaxf(m, ml[i].x), f = exp2_approx(m - m2), w = exp2_approx(ml[i].x - m2);
+          m = m2;
+          l = l * f + ml[i].y * w;
+#pragma unroll
+          for (int v = 0; v < V; v++) o[v] = o[v] * f + x[i][v] * w;
+        }
+      }
+    }
+    if (WPR > 1) {
+#pragma unroll
+      for (int v = 0; v < V; v++) s_o[warp][V * lane + v] = o[v];
+      if (lane == 0) s_ml[warp] = make_float2(m, l);
+      __syncthreads();
+      if (sub == 0) {
+#pragma unroll
+        for (int i = 1; i < WPR; i++) {
+          const float2 z = s_ml[warp + i];
+          if (z.x == -INFINITY) continue;
+          const float m2 = fmaxf(m, z.x), f = exp2_approx(m - m2), w = exp2_approx(z.x - m2);
+          m = m2;
+          l = l * f + z.y * w;
+#pragma unroll
+          for (int v = 0; v < V; v++) o[v] = o[v] * f + s_o[warp + i][V * lane + v] * w;
+        }
+      }
+      __syncthreads();
+    }
+    if (!live || sub != 0) continue;
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
+    const long long tk = cut.t0 + tok;
+    uint16_t *op = c.out + tk * c.o_st + head * c.o_sh + V * lane;
+#pragma unroll
+    for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t *>(op + v) = pack2<F16>(o[v] * inv, o[v + 1] * inv);
+    if (c.lse && lane == 0) c.lse[tk * c.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  }
+}
+
 // ------------------------------------------------------------------ host ---
+// A launch that may come up before its predecessor in the stream has ended (it
+// calls pdl_wait before it reads that one's results).
+template <typename... P, typename... A>
+static cudaError_t launch_early(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 typedef CUresult (*TensorMapFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
                                 const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

@@ -47,7 +47,6 @@ _this_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream   # what torch.cuda.current_stream(i).cuda_stream is, without the object
 
 _calls = None
-_workspace = {}              # bytes by (device, head_dim, paged?, positive scale?)
 
 
 def _lib():
@@ -191,15 +190,13 @@ def _attend(q, k, v, cu, kv_len, table, pool, max_new, max_kv, scale, causal, wi
             0 if status is None else _index("status", status, dev, 1))
     tail = (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2] if pool else 0, vs[0], vs[1], vs[2] if pool else 0,
             width, cols, page, pages, n, t, h, kv, d, max_new, max_kv, _TYPES[kind], causal, window or 0, scale)
-    key = (dev, d, pool, scale > 0)          # what the workspace's size depends on
-    size = _workspace.get(key)
-    if size is None:
+    if dev == _this_device():
+        size = L.qtb_attn_workspace(_ATTN(*head, 0, 0, *tail), pool)
+    else:
         with torch.cuda.device(dev):
             size = L.qtb_attn_workspace(_ATTN(*head, 0, 0, *tail), pool)
-        if size < 0:
-            Q.check(size)
-        if n and t:
-            _workspace[key] = size
+    if size < 0:
+        Q.check(size)
     at, ws = 0, None
     if size:
         ws = q.new_empty(size // 2)          # of two-byte values
