@@ -438,7 +438,7 @@ static cudaError_t rows_run(bool prepare, const AttnCall *c, const RowsMaps *m, 
   float *parts = reinterpret_cast<float *>(cuts + grid);
   rows_kernel<HD, F16, PAGED><<<grid, ROWS_THREADS, rows_smem<HD>(), st>>>(*c, *m, row_limit, rows_box(PAGED, c->page), parts, cuts);
   if (cudaError_t e = cudaGetLastError()) return e;
-  return launch_early(join_kernel<HD, F16, ROWS_M, 1, JOIN_WARPS>, dim3(grid, max_rows), 32 * JOIN_WARPS, 0, st, *c, (const float *)parts,
+  return launch_early(join_kernel<HD, F16, ROWS_M, 1, JOIN_WARPS, 1>, dim3(grid, max_rows), 32 * JOIN_WARPS, 0, st, *c, (const float *)parts,
                       (const AttnCut *)cuts);
 }
 // Requests with at most row_limit query rows to a key head are served; max_rows

@@ -25,13 +25,15 @@
 // The probabilities of a tile start from the old maximum at once, beside the new
 // maximum's search, and are thrown away in the rare tile that outgrows it.
 //
-// An item of work is a tile pair and a key head.  Where there are many to a
-// block, they are dealt out whole, longest first.  Where there are few, the key
-// tiles of all are dealt out in equal runs, whatever the requests' lengths; an
-// item that is cut between blocks leaves its parts in the workspace, and
-// join_kernel adds them.  (Runs of many items would also walk the keys at as
-// many places at once as there are blocks: a prompt of 16384 tokens, 16 / 8
-// heads, took 993 us so, and 827 us with whole items.)
+// An item of work is a tile pair and a key head.  Where whole items fill the
+// blocks evenly enough (2.5 to a block, or one to at least three of four), they
+// are dealt out whole, longest first.  Where not, the key tiles of all are dealt
+// out in equal runs, whatever the requests' lengths; an item that is cut between
+// blocks leaves its parts in the workspace, and join_kernel adds them.  Cutting
+// costs the parts, the join and the key tiles' reuse in L2, since blocks then walk
+// the keys at as many places as there are blocks (us, whole / cut: 8192-token
+// prompt, 512 items, 212 / 272; 4 x 512 tokens over 8192 keys, 128 items, 122 /
+// 137; 8 x 64 tokens over 8192 keys, 64 items, 133 / 75).
 //
 // Products are issued in order, so the commit that completes S of tile j also
 // says that P V of tile j - 1 is in O: the softmax warps may scale O then.
@@ -47,8 +49,7 @@ constexpr int TILE_THREADS = 384, TILE_M = 128, TILE_N = 128;
 // (64512 in all); the softmax warps, a row of S each, take what the loading and
 // issuing warpgroup gives up: 256 * 200 + 128 * 96 = 63488.
 constexpr int TILE_REGS_SOFTMAX = 200, TILE_REGS_OTHER = 96;
-constexpr int TILE_DEAL = 4;               // items to a block from which on they are dealt out whole
-constexpr int TILE_CUT = 2;                // key tiles that a block has of an item at least, where it has not all
+constexpr int TILE_CUT = 1;                // key tiles that a block has of an item at least, where it has not all
 constexpr int TILE_SEGS = 128;             // runs of requests that the in-block search tells apart
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
@@ -215,6 +216,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   unsigned char *s_q = smem, *s_kv = smem + 2 * Q_B;
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // known to be the same in the whole warp
+  if (parts) pdl_release();                // the join kernel's blocks may come up; they wait for this grid's end
   if (warp == 8) {
     if (lane < 3) {
       const CUtensorMap *m = lane == 0 ? &maps.q : lane == 1 ? &maps.k : &maps.v;
@@ -301,7 +303,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   // started; boundaries between blocks move to an item's start or end where less
   // than TILE_CUT key tiles would be left on that side.
   const int items = pairs * c.n_kv;        // the host has bounded it
-  const bool deal = !parts || items >= TILE_DEAL * (int)gridDim.x;
+  const int grid = (int)gridDim.x;
+  const bool deal = !parts || 2 * (long long)items >= 5 * grid || (items <= grid && 4 * items >= 3 * grid);
   if (deal) {
     if (tid == 0 && parts) cuts[blockIdx.x].last = -1;
   } else {
@@ -383,7 +386,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   auto get_item = [&](int n, TileItem &it) {
     int i, from = 0, off1 = 0;
     if (deal) {
-      i = n * (int)gridDim.x + (int)(n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+      i = n * grid + (n & 1 ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
       if (i >= items) return false;
     } else {
       i = sh.item[0] + n;
@@ -425,6 +428,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     int bad = 0;
     uint32_t fill = 0, n_items = 0;        // ring fills issued; items begun
     bool ok = true;
+#pragma unroll 1
     for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
@@ -442,6 +446,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
         n_items++;
         return true;
       };
+#pragma unroll 1
       for (int j = it.from; j < to && ok; j++) {
         const int kb = it.k0 + j * TILE_N;
         // this lane's box of the key tile: positions [pos, pos + box), 64 dims
@@ -489,6 +494,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     // descriptors of the first tile and stage: others are an address (in 16 bytes) further on
     const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_kv));
     const uint64_t v_desc = umma_desc_mn128(smem_u32(s_kv), HALF_B);
+#pragma unroll 1
     for (int i = 0; ok; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
@@ -520,6 +526,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       }
       __syncwarp();
       fill++;
+#pragma unroll 1
       for (int j = it.from; j < to && ok; j++) {
         const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
         const bool more = j + 1 < to;
@@ -578,6 +585,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
     const uint32_t s_at = tmem + S_COL + t * 128 + lanes, o_at = tmem + O_COL + t * HD + lanes;
     uint32_t fill = 0, s_n = 0, o_n = 0;
+#pragma unroll 1
     for (int i = 0;; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
@@ -593,6 +601,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
       const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
       float m = -INFINITY, l = 0.f;
       bool ok = true;
+#pragma unroll 1
       for (int j = it.from; j < n; j++) {
         if (!(ok = wait(&sy.s_full[t], s_n & 1))) break;
         s_n++;
@@ -829,7 +838,7 @@ static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, 
   float *parts = reinterpret_cast<float *>(cuts + sms);
   tile_kernel<HD, F16, PAGED><<<sms, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tpt, box, parts, cuts);
   if (cudaError_t e = cudaGetLastError()) return e;
-  return launch_early(join_kernel<HD, F16, TILE_M, 2, 1>, dim3(sms, 2 * TILE_M / JOIN_WARPS), 32 * JOIN_WARPS, 0, st, *c,
+  return launch_early(join_kernel<HD, F16, TILE_M, 2, 1, 4>, dim3(sms, 2 * TILE_M / (4 * JOIN_WARPS)), 32 * JOIN_WARPS, 0, st, *c,
                       (const float *)parts, (const AttnCut *)cuts);
 }
 static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int sms, int row_limit, void *ws,

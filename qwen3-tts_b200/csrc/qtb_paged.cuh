@@ -116,11 +116,14 @@ constexpr int JOIN_WARPS = 8;
 
 // Adds the parts of the item that block blockIdx.x cut: part 1 of that block,
 // then part 0 of the following ones.  WPR warps share a row (they take every
-// WPR-th part and join theirs in warp order), a lane has HD / 32 of its dims.
-template <int HD, bool F16, int M, int TILES, int WPR>
+// WPR-th part and join theirs in warp order), or a warp has RPW rows side by
+// side; a lane has HD / 32 dims of each.  Bounded by the latency of a part's
+// loads: those of UNROLL parts of all its rows are in flight together.
+template <int HD, bool F16, int M, int TILES, int WPR, int RPW>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 join_kernel(const AttnCall c, const float *__restrict__ parts, const AttnCut *__restrict__ cuts) {
-  constexpr int TF = M * (HD + 2), V = HD / 32, UNROLL = 4, ROWS = JOIN_WARPS / WPR;
+  static_assert(WPR == 1 || RPW == 1, "rows of a warp");
+  constexpr int TF = M * (HD + 2), V = HD / 32, UNROLL = RPW > 1 ? 2 : 4, ROWS = JOIN_WARPS / WPR * RPW;
   __shared__ float s_o[WPR > 1 ? JOIN_WARPS : 1][HD];
   __shared__ float2 s_ml[JOIN_WARPS];
   pdl_wait();
@@ -128,64 +131,83 @@ join_kernel(const AttnCall c, const float *__restrict__ parts, const AttnCut *__
   if (cut.last < 0) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, b0 = blockIdx.x, n = cut.last - b0 + 1, sub = warp % WPR;
   for (int r0 = blockIdx.y * ROWS; r0 < M * TILES; r0 += gridDim.y * ROWS) {
-    const int row = r0 + warp / WPR, tile = row / M, rr = row - tile * M;
-    const int at = cut.row0 + tile * cut.per_tile + rr, tok = at / c.group, head = cut.head0 + at - tok * c.group;
-    const bool live = rr < cut.per_tile && tok < cut.n;
-    if (WPR > 1 && !live) return;          // the whole block's row
-    float m = -INFINITY, l = 0.f, o[V] = {};
-    if (live) {
-      auto part = [&](int i) { return parts + ((long long)(2 * (b0 + i) + (i == 0 ? 1 : 0)) * TILES + tile) * TF; };
-      for (int i0 = sub; i0 < n; i0 += WPR * UNROLL) {
-        float x[UNROLL][V];
-        float2 ml[UNROLL];
+    const int row = r0 + warp / WPR * RPW, tile = row / M, rr = row - tile * M;
+    const float *base = parts + (long long)(2 * b0) * TILES * TF + tile * TF + rr * HD + V * lane;   // part 0 of b0
+    const float *base_ml = parts + (long long)(2 * b0) * TILES * TF + tile * TF + M * HD + 2 * rr;
+    const int at0 = cut.row0 + tile * cut.per_tile + rr;
+    if (rr >= cut.per_tile || at0 / c.group >= cut.n) {   // the rows of a warp run on: its first one tells
+      if (WPR > 1) return;                 // all warps have this row
+      continue;
+    }
+    float m[RPW], l[RPW], o[RPW][V];
 #pragma unroll
-        for (int i = 0; i < UNROLL; i++) {
-          const float *p = part(min(i0 + i * WPR, n - 1));
-          ml[i] = *reinterpret_cast<const float2 *>(p + M * HD + 2 * rr);
+    for (int r = 0; r < RPW; r++) {
+      m[r] = -INFINITY;
+      l[r] = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; v++) o[r][v] = 0.f;
+    }
+    for (int i0 = sub; i0 < n; i0 += WPR * UNROLL) {
+      float x[UNROLL][RPW][V];
+      float2 ml[UNROLL][RPW];
+#pragma unroll
+      for (int i = 0; i < UNROLL; i++) {
+        const int k = min(i0 + i * WPR, n - 1);
+        const long long off = (long long)(2 * k + (k == 0 ? 1 : 0)) * TILES * TF;
+#pragma unroll
+        for (int r = 0; r < RPW; r++) {
+          ml[i][r] = *reinterpret_cast<const float2 *>(base_ml + off + 2 * r);
 #pragma unroll
           for (int v = 0; v < V; v += 2) {
-            const float2 y = *reinterpret_cast<const float2 *>(p + rr * HD + V * lane + v);
-            x[i][v] = y.x; x[i][v + 1] = y.y;
+            const float2 y = *reinterpret_cast<const float2 *>(base + off + r * HD + v);
+            x[i][r][v] = y.x; x[i][r][v + 1] = y.y;
           }
         }
-#pragma unroll
-        for (int i = 0; i < UNROLL; i++) {
-          // a part without a visible key has m = -inf, and O that was never written
-          if (i0 + i * WPR >= n || ml[i].x == -INFINITY) continue;
-          const float m2 = fmaxf(m, ml[i].x), f = exp2_approx(m - m2), w = exp2_approx(ml[i].x - m2);
-          m = m2;
-          l = l * f + ml[i].y * w;
-#pragma unroll
-          for (int v = 0; v < V; v++) o[v] = o[v] * f + x[i][v] * w;
-        }
       }
+#pragma unroll
+      for (int i = 0; i < UNROLL; i++)
+#pragma unroll
+        for (int r = 0; r < RPW; r++) {
+          // a part without a visible key has m = -inf, and O that was never written
+          if (i0 + i * WPR >= n || ml[i][r].x == -INFINITY) continue;
+          const float m2 = fmaxf(m[r], ml[i][r].x), f = exp2_approx(m[r] - m2), w = exp2_approx(ml[i][r].x - m2);
+          m[r] = m2;
+          l[r] = l[r] * f + ml[i][r].y * w;
+#pragma unroll
+          for (int v = 0; v < V; v++) o[r][v] = o[r][v] * f + x[i][r][v] * w;
+        }
     }
     if (WPR > 1) {
 #pragma unroll
-      for (int v = 0; v < V; v++) s_o[warp][V * lane + v] = o[v];
-      if (lane == 0) s_ml[warp] = make_float2(m, l);
+      for (int v = 0; v < V; v++) s_o[warp][V * lane + v] = o[0][v];
+      if (lane == 0) s_ml[warp] = make_float2(m[0], l[0]);
       __syncthreads();
       if (sub == 0) {
 #pragma unroll
         for (int i = 1; i < WPR; i++) {
           const float2 z = s_ml[warp + i];
           if (z.x == -INFINITY) continue;
-          const float m2 = fmaxf(m, z.x), f = exp2_approx(m - m2), w = exp2_approx(z.x - m2);
-          m = m2;
-          l = l * f + z.y * w;
+          const float m2 = fmaxf(m[0], z.x), f = exp2_approx(m[0] - m2), w = exp2_approx(z.x - m2);
+          m[0] = m2;
+          l[0] = l[0] * f + z.y * w;
 #pragma unroll
-          for (int v = 0; v < V; v++) o[v] = o[v] * f + s_o[warp + i][V * lane + v] * w;
+          for (int v = 0; v < V; v++) o[0][v] = o[0][v] * f + s_o[warp + i][V * lane + v] * w;
         }
       }
       __syncthreads();
+      if (sub != 0) continue;
     }
-    if (!live || sub != 0) continue;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
-    const long long tk = cut.t0 + tok;
-    uint16_t *op = c.out + tk * c.o_st + head * c.o_sh + V * lane;
 #pragma unroll
-    for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t *>(op + v) = pack2<F16>(o[v] * inv, o[v + 1] * inv);
-    if (c.lse && lane == 0) c.lse[tk * c.n_heads + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    for (int r = 0; r < RPW; r++) {
+      const int at = at0 + r, tok = at / c.group, head = cut.head0 + at - tok * c.group;
+      if (rr + r >= cut.per_tile || tok >= cut.n) continue;
+      const float inv = l[r] > 0.f || l[r] != l[r] ? 1.f / l[r] : 0.f;   // no visible key: zeros
+      const long long tk = cut.t0 + tok;
+      uint16_t *op = c.out + tk * c.o_st + head * c.o_sh + V * lane;
+#pragma unroll
+      for (int v = 0; v < V; v += 2) *reinterpret_cast<uint32_t *>(op + v) = pack2<F16>(o[r][v] * inv, o[r][v + 1] * inv);
+      if (c.lse && lane == 0) c.lse[tk * c.n_heads + head] = l[r] == 0.f ? -INFINITY : (m[r] + log2f(l[r])) * 0.6931471805599453f;
+    }
   }
 }
 
