@@ -35,7 +35,8 @@ enum {
     QTB_E_OOM = -3,       /* device allocation failed */
     QTB_E_DEVICE = -4,    /* the decode kernel raised its error flag (bounded wait
                              expired or an index failed its device-side check) */
-    QTB_E_UNSUPPORTED = -5
+    QTB_E_UNSUPPORTED = -5,
+    QTB_E_WORKSPACE = -6  /* the call needs a workspace, or a larger one (qtb_attn_workspace) */
 };
 
 /* Weight storage formats.  One format per transformer (the reference picks one

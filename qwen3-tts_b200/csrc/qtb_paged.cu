@@ -363,8 +363,9 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   if ((rc = device_info(&dev))) return rc;
   const AttnPlan p = attn_plan(c, d, paged, dev->sms);
   const int64_t need = (int64_t)p.ws;
-  if (d->workspace_bytes < need || (need && !d->workspace) || !aligned16(d->workspace))
-    return qtb_fail(QTB_E_INVALID, "workspace of %lld bytes on 16: %lld needed", (long long)d->workspace_bytes, (long long)need);
+  if (d->workspace_bytes < need || (need && !d->workspace))
+    return qtb_fail(QTB_E_WORKSPACE, "workspace of %lld bytes: %lld needed", (long long)d->workspace_bytes, (long long)need);
+  if (!aligned16(d->workspace)) return qtb_fail(QTB_E_INVALID, "the workspace must start on 16 bytes");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == QTB_T_F16;
   const int hd = (int)d->head_dim;

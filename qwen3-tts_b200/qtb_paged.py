@@ -40,12 +40,14 @@ _PLAN = struct.Struct("12Q6q").pack       # qtb_paged_plan_t
 _APPEND = struct.Struct("6Q17q").pack     # qtb_paged_append_t
 _ATTN = struct.Struct("10Q25qd").pack     # qtb_attn_t
 
-# A call's host side is a few microseconds of Python next to kernels of as many:
-# the checks below are flat on purpose.
+# A call's host side is a few microseconds of Python beside kernels of as many, so
+# each function checks all of its tensors in one condition, and names what is wrong
+# (_refuse) only when that fails.
 _i32, _i64, _f32 = torch.int32, torch.int64, torch.float32
 _this_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream   # what torch.cuda.current_stream(i).cuda_stream is, without the object
 
+_NEEDS = -6                 # QTB_E_WORKSPACE
 _calls = None
 
 
@@ -61,39 +63,25 @@ def _lib():
     return _calls
 
 
-def _call(dev: int, fn, desc: bytes):
-    """fn(desc, stream) on the current stream of device `dev`."""
+def _on_device(dev: int, fn, *args):
     if dev == _this_device():
-        rc = fn(desc, _stream_of(dev))
-    else:
-        with torch.cuda.device(dev):
-            rc = fn(desc, _stream_of(dev))
-    if rc:
-        Q.check(rc)
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
 
 
-def _refuse(name, want, t):
-    raise ValueError(f"{name}: {want} wanted, got {t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-
-
-def _index(name, t, dev, n=None, dtype=_i32):
-    """Pointer of a contiguous one-dimensional index tensor of `n` elements."""
-    if t.dtype is not dtype or t.get_device() != dev or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-        _refuse(name, f"contiguous {dtype} [{'*' if n is None else n}] on cuda:{dev}", t)
-    return t.data_ptr()
-
-
-def _table(table, dev, n):
-    if table.dtype is not _i32 or table.get_device() != dev or table.dim() != 2 or table.shape[0] != n or (
-            table.shape[1] > 1 and table.stride(1) != 1):
-        _refuse("table", f"int32 [{n}][columns] with contiguous rows on cuda:{dev}", table)
-    return table.data_ptr()
-
-
-def _cuda(t):
-    if not t.is_cuda:
-        raise ValueError(f"CUDA tensors wanted, got one on {t.device}")
-    return t.get_device()
+def _refuse(dev, *wanted):
+    """Raise for the first tensor that is not as wanted: (name, tensor, dtype, shape with None for any extent)."""
+    for name, t, dtype, shape in wanted:
+        if t is None:
+            continue
+        if not (t.is_cuda and t.get_device() == dev and t.dtype is dtype and t.dim() == len(shape)
+                and all(w is None or w == s for w, s in zip(shape, t.shape)) and (t.dim() == 0 or t.stride(-1) == 1 or t.shape[-1] < 2)
+                and (t.dim() != 1 or t.is_contiguous())):
+            dims = "".join("[*]" if w is None else f"[{w}]" for w in shape)
+            raise ValueError(f"{name}: {dtype} {dims}, contiguous in its last dimension, on cuda:{dev} wanted, got {t.dtype} "
+                             f"{tuple(t.shape)} with strides {t.stride()} on {t.device}")
+    raise ValueError("tensors that do not go together")
 
 
 class Plan(NamedTuple):
@@ -112,19 +100,28 @@ def plan(past_len, new_len, table, free_pages, page: int, max_tokens: int, free_
     [requests][columns], its rows hold the pages of the cached tokens and
     receive those of the new ones, taken in request order from free_pages
     (int32) at free_head (int32 [1], default 0; pass the last plan's)."""
-    dev = _cuda(past_len)
-    n = past_len.shape[0]
+    dev = past_len.get_device()
+    n = past_len.numel()
+    cols = table.shape[-1]
+    if not (dev >= 0 and past_len.dtype is new_len.dtype is table.dtype is free_pages.dtype is _i32
+            and past_len.shape == new_len.shape == (n,) and table.shape == (n, cols) and free_pages.dim() == 1
+            and new_len.get_device() == table.get_device() == free_pages.get_device() == dev
+            and past_len.is_contiguous() and new_len.is_contiguous() and free_pages.is_contiguous()
+            and (cols < 2 or table.stride(1) == 1)
+            and (free_head is None or free_head.dtype is _i32 and free_head.shape == (1,) and free_head.get_device() == dev)
+            and (status is None or status.dtype is _i32 and status.shape == (1,) and status.get_device() == dev)):
+        _refuse(dev, ("past_len", past_len, _i32, (n,)), ("new_len", new_len, _i32, (n,)), ("table", table, _i32, (n, None)),
+                ("free_pages", free_pages, _i32, (None,)), ("free_head", free_head, _i32, (1,)), ("status", status, _i32, (1,)))
     ints = past_len.new_empty(2 * n + 2 + 2 * max_tokens)
     slot = past_len.new_empty(max_tokens, dtype=_i64)
-    if ints.dtype is not _i32:
-        _refuse("past_len", "int32", past_len)
     at = ints.data_ptr()
-    _call(dev, _lib().qtb_paged_plan, _PLAN(
-        _index("past_len", past_len, dev), _index("new_len", new_len, dev, n), _table(table, dev, n),
-        _index("free_pages", free_pages, dev), 0 if free_head is None else _index("free_head", free_head, dev, 1),
-        at, at + 4 * n + 4, slot.data_ptr(), at + 8 * n + 8, at + 8 * n + 8 + 4 * max_tokens, at + 8 * n + 4,
-        0 if status is None else _index("status", status, dev, 1),
-        n, max_tokens, table.shape[1], table.stride(0), free_pages.shape[0], page))
+    rc = _on_device(dev, _lib().qtb_paged_plan, _PLAN(
+        past_len.data_ptr(), new_len.data_ptr(), table.data_ptr(), free_pages.data_ptr(),
+        0 if free_head is None else free_head.data_ptr(), at, at + 4 * n + 4, slot.data_ptr(), at + 8 * n + 8,
+        at + 8 * n + 8 + 4 * max_tokens, at + 8 * n + 4, 0 if status is None else status.data_ptr(),
+        n, max_tokens, cols, table.stride(0), free_pages.shape[0], page), _stream_of(dev))
+    if rc:
+        Q.check(rc)
     cu, kv, head, pos, req = torch.split_with_sizes(ints, (n + 1, n, 1, max_tokens, max_tokens))
     return Plan(cu, kv, slot, pos, req, head)
 
@@ -135,74 +132,54 @@ def append(k, v, kpool, vpool, slot, status=None) -> None:
     k, v: [tokens][heads][dim] of the pools' type or f32 (rounded to nearest
     even); slot: int64 [tokens], negative = skip.  Pools: bf16 or f16
     [pages][heads][position][dim], updated in place."""
-    dev = _cuda(k)
-    t, h, d = k.shape
-    src, dst, pools = k.dtype, kpool.dtype, kpool.shape
-    if src not in _TYPES or dst not in _TYPES:
-        raise ValueError(f"append: {src} into {dst} is not supported")
-    if v.dtype is not src or v.get_device() != dev or v.shape != k.shape:
-        _refuse("v", f"{src} {tuple(k.shape)} on cuda:{dev}", v)
-    if kpool.get_device() != dev or len(pools) != 4 or pools[1] != h or pools[3] != d:
-        _refuse("kpool", f"[pages][{h}][position][{d}] on cuda:{dev}", kpool)
-    if vpool.dtype is not dst or vpool.get_device() != dev or vpool.shape != pools:
-        _refuse("vpool", f"{dst} {tuple(pools)} on cuda:{dev}", vpool)
+    dev = k.get_device()
+    t, h, d = shape = k.shape
+    pages, _, page, _ = pools = kpool.shape
+    src, dst = k.dtype, kpool.dtype
     ks, vs, kp, vp = k.stride(), v.stride(), kpool.stride(), vpool.stride()
-    if not ks[2] == vs[2] == kp[3] == vp[3] == 1:
-        raise ValueError("append: the last dimension has to be contiguous")
-    _call(dev, _lib().qtb_paged_append, _APPEND(
-        k.data_ptr(), v.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), _index("slot", slot, dev, t, _i64),
-        0 if status is None else _index("status", status, dev, 1), ks[0], ks[1], vs[0], vs[1],
-        kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], t, h, d, pools[2], pools[0], _TYPES[src], _TYPES[dst]))
+    if not (dev >= 0 and src in _TYPES and dst in _TYPES and v.dtype is src and vpool.dtype is dst and slot.dtype is _i64
+            and v.shape == shape and pools[1] == h and pools[3] == d and vpool.shape == pools and slot.shape == (t,)
+            and v.get_device() == kpool.get_device() == vpool.get_device() == slot.get_device() == dev
+            and ks[2] == vs[2] == kp[3] == vp[3] == 1 and slot.is_contiguous()
+            and (status is None or status.dtype is _i32 and status.shape == (1,) and status.get_device() == dev)):
+        _refuse(dev, ("k", k, src if src in _TYPES else _f32, (t, h, d)), ("v", v, src, (t, h, d)),
+                ("kpool", kpool, dst if dst in _TYPES else torch.bfloat16, (None, h, None, d)), ("vpool", vpool, dst, tuple(pools)),
+                ("slot", slot, _i64, (t,)), ("status", status, _i32, (1,)))
+    rc = _on_device(dev, _lib().qtb_paged_append, _APPEND(
+        k.data_ptr(), v.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), slot.data_ptr(), 0 if status is None else status.data_ptr(),
+        ks[0], ks[1], vs[0], vs[1], kp[0], kp[1], kp[2], vp[0], vp[1], vp[2], t, h, d, page, pages, _TYPES[src], _TYPES[dst]),
+        _stream_of(dev))
+    if rc:
+        Q.check(rc)
 
 
-def _attend(q, k, v, cu, kv_len, table, pool, max_new, max_kv, scale, causal, window, out, lse, status):
-    dev = _cuda(q)
-    t, h, d = q.shape
-    kind, n = q.dtype, cu.shape[0] - 1
-    if kind not in _TYPES:
-        raise ValueError(f"attention of {kind} is not supported")
-    if k.dtype is not kind or k.get_device() != dev or k.dim() != 3 + pool or k.shape[-1] != d or (not pool and k.shape[0] != t):
-        _refuse("kpool" if pool else "k", f"{kind} " + (f"[pages][head][position][{d}]" if pool else f"[{t}][head][{d}]") + f" on cuda:{dev}", k)
-    if v.dtype is not kind or v.get_device() != dev or v.shape != k.shape:
-        _refuse("vpool" if pool else "v", f"{kind} {tuple(k.shape)} on cuda:{dev}", v)
-    qs, ks, vs = q.stride(), k.stride(), v.stride()
-    if pool:
-        pages, kv, page, _ = k.shape
-        lens, rows, cols, width = _index("kv_len", kv_len, dev, n), _table(table, dev, n), table.shape[1], table.stride(0)
-    else:
-        kv = k.shape[1]
-        pages = page = lens = rows = cols = width = 0
+def _results(q, out, lse, status, dev):
+    """out and lse of a call: those given, checked, or new ones."""
     if out is None:
-        out = q.new_empty((t, h, d))
-    elif out.dtype is not kind or out.get_device() != dev or out.shape != q.shape:
-        _refuse("out", f"{kind} {tuple(q.shape)} on cuda:{dev}", out)
-    os = out.stride()
-    if not qs[2] == ks[-1] == vs[-1] == os[2] == 1:
-        raise ValueError("attention: the last dimension has to be contiguous")
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
+    elif not (out.dtype is q.dtype and out.shape == q.shape and out.stride(2) == 1 and out.get_device() == dev):
+        _refuse(dev, ("out", out, q.dtype, tuple(q.shape)))
     if lse is None:
-        lse = q.new_empty((t, h), dtype=_f32)
-    elif lse.dtype is not _f32 or lse.get_device() != dev or lse.shape != (t, h) or not lse.is_contiguous():
-        _refuse("lse", f"contiguous float32 [{t}][{h}] on cuda:{dev}", lse)
-    if scale is None:
-        scale = 1 / math.sqrt(d)
-    L = _lib()
-    head = (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), _index("cu_new", cu, dev), lens, rows,
-            0 if status is None else _index("status", status, dev, 1))
-    tail = (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2] if pool else 0, vs[0], vs[1], vs[2] if pool else 0,
-            width, cols, page, pages, n, t, h, kv, d, max_new, max_kv, _TYPES[kind], causal, window or 0, scale)
-    if dev == _this_device():
-        size = L.qtb_attn_workspace(_ATTN(*head, 0, 0, *tail), pool)
-    else:
-        with torch.cuda.device(dev):
-            size = L.qtb_attn_workspace(_ATTN(*head, 0, 0, *tail), pool)
-    if size < 0:
-        Q.check(size)
-    at, ws = 0, None
-    if size:
-        ws = q.new_empty(size // 2)          # of two-byte values
-        at = ws.data_ptr()
-    _call(dev, L.qtb_paged_attention if pool else L.qtb_prompt_attention, _ATTN(*head, at, size, *tail))
+        lse = q.new_empty(q.shape[:2], dtype=_f32)
+    elif not (lse.dtype is _f32 and lse.shape == q.shape[:2] and lse.is_contiguous() and lse.get_device() == dev):
+        raise ValueError(f"lse: contiguous {_f32} {tuple(q.shape[:2])} on cuda:{dev} wanted, got {lse.dtype} {tuple(lse.shape)} with "
+                         f"strides {lse.stride()} on {lse.device}")
+    if status is not None and not (status.dtype is _i32 and status.shape == (1,) and status.get_device() == dev):
+        _refuse(dev, ("status", status, _i32, (1,)))
     return out, lse
+
+
+def _attend(fn, pool, dev, q, head, tail):
+    """One attention call, and the workspace that it says it needs."""
+    rc = _NEEDS if pool else _on_device(dev, fn, _ATTN(*head, 0, 0, *tail), _stream_of(dev))
+    if rc == _NEEDS:
+        size = _on_device(dev, _lib().qtb_attn_workspace, _ATTN(*head, 0, 0, *tail), pool)
+        if size < 0:
+            Q.check(size)
+        ws = q.new_empty(size // 2)              # of two-byte values
+        rc = _on_device(dev, fn, _ATTN(*head, ws.data_ptr(), size, *tail), _stream_of(dev))
+    if rc:
+        Q.check(rc)
 
 
 def paged_attention(q, kpool, vpool, table, cu_new, kv_len, max_new: int = 0, max_kv: int = 0, scale=None,
@@ -214,14 +191,50 @@ def paged_attention(q, kpool, vpool, table, cu_new, kv_len, max_new: int = 0, ma
     window: how many keys a token looks back on, itself included (0: all).
     max_new, max_kv: bounds of new tokens and keys per request, to choose the
     split of the work (0: not known).  Returns (out, lse)."""
-    return _attend(q, kpool, vpool, cu_new, kv_len, table, True, max_new, max_kv, scale, causal, window, out, lse, status)
+    dev = q.get_device()
+    t, h, d = q.shape
+    pages, kv, page, _ = pools = kpool.shape
+    n, cols, kind = kv_len.numel(), table.shape[-1], q.dtype
+    qs, ks, vs = q.stride(), kpool.stride(), vpool.stride()
+    if not (dev >= 0 and kind in _TYPES and kpool.dtype is vpool.dtype is kind and table.dtype is cu_new.dtype is kv_len.dtype is _i32
+            and pools[3] == d and vpool.shape == pools and table.shape == (n, cols) and cu_new.shape == (n + 1,) and kv_len.dim() == 1
+            and kpool.get_device() == vpool.get_device() == table.get_device() == cu_new.get_device() == kv_len.get_device() == dev
+            and qs[2] == ks[3] == vs[3] == 1 and (cols < 2 or table.stride(1) == 1) and cu_new.is_contiguous() and kv_len.is_contiguous()):
+        _refuse(dev, ("q", q, kind if kind in _TYPES else torch.bfloat16, (t, h, d)), ("kpool", kpool, kind, (None, None, None, d)),
+                ("vpool", vpool, kind, tuple(pools)), ("table", table, _i32, (n, None)), ("cu_new", cu_new, _i32, (n + 1,)),
+                ("kv_len", kv_len, _i32, (n,)))
+    out, lse = _results(q, out, lse, status, dev)
+    os = out.stride()
+    _attend(_lib().qtb_paged_attention, 1, dev, q,
+            (q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_new.data_ptr(), kv_len.data_ptr(),
+             table.data_ptr(), 0 if status is None else status.data_ptr()),
+            (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.stride(0), cols, page, pages, n, t, h, kv, d,
+             max_new, max_kv, _TYPES[kind], causal, window or 0, 1 / math.sqrt(d) if scale is None else scale))
+    return out, lse
 
 
 def prompt_attention(q, k, v, cu_new, max_new: int = 0, scale=None, causal: bool = True, window: int = 0, out=None,
                      lse=None, status=None):
     """Attention within packed prompts (qtb_prompt_attention): q [tokens][heads]
     [dim], k and v [tokens][key heads][dim].  Returns (out, lse)."""
-    return _attend(q, k, v, cu_new, None, None, False, max_new, max_new, scale, causal, window, out, lse, status)
+    dev = q.get_device()
+    t, h, d = q.shape
+    kv, n, kind = k.shape[1], cu_new.numel() - 1, q.dtype
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if not (dev >= 0 and n >= 0 and kind in _TYPES and k.dtype is v.dtype is kind and cu_new.dtype is _i32
+            and k.shape == v.shape == (t, kv, d) and cu_new.dim() == 1
+            and k.get_device() == v.get_device() == cu_new.get_device() == dev
+            and qs[2] == ks[2] == vs[2] == 1 and cu_new.is_contiguous()):
+        _refuse(dev, ("q", q, kind if kind in _TYPES else torch.bfloat16, (t, h, d)), ("k", k, kind, (t, None, d)), ("v", v, kind, (t, kv, d)),
+                ("cu_new", cu_new, _i32, (None,)))
+    out, lse = _results(q, out, lse, status, dev)
+    os = out.stride()
+    _attend(_lib().qtb_prompt_attention, 0, dev, q,
+            (q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_new.data_ptr(), 0, 0,
+             0 if status is None else status.data_ptr()),
+            (qs[0], qs[1], os[0], os[1], ks[0], ks[1], 0, vs[0], vs[1], 0, 0, 0, 0, 0, n, t, h, kv, d,
+             max_new, max_new, _TYPES[kind], causal, window or 0, 1 / math.sqrt(d) if scale is None else scale))
+    return out, lse
 
 
 def check_status(status) -> None:
