@@ -79,7 +79,10 @@ struct TileSync {
 struct TileShared {
   TileSync sy;
   int pre[TILE_SEGS + 1];                  // query tile pairs before each run of requests
-  int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS];   // the requests themselves, where a run is one
+  // the requests themselves, where a run is one: in order of their keys, so that
+  // items taken from the last to the first begin with the longest
+  int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS];
+  unsigned char r[TILE_SEGS];
   long long scan[TILE_THREADS / 32];
   int item[2], off[2];                     // the block's first item and place in it, and where the next block's are
   long long base;                          // units of work before item[1]
@@ -239,12 +242,28 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
   const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS;
   auto pairs_of = [&](int n) { return n * c.group > row_limit ? (n + 2 * tpt - 1) / (2 * tpt) : 0; };
   int sum = 0, pre = 0;
-  if (tid < TILE_SEGS) {
-    for (int r = tid * seg; r < min((tid + 1) * seg, c.n_req); r++) {
-      const AttnReq a = attn_request<PAGED>(c, r);
-      sum += pairs_of(a.n);
-      sh.t0[tid] = a.t0; sh.n[tid] = a.n; sh.hi[tid] = a.hi;
+  if (seg > 1) {
+    if (tid < TILE_SEGS)
+      for (int r = tid * seg; r < min((tid + 1) * seg, c.n_req); r++) sum += pairs_of(attn_request<PAGED>(c, r).n);
+  } else {
+    AttnReq a = {};
+    int place = tid;
+    if (tid < c.n_req) a = attn_request<PAGED>(c, tid);
+    if (c.n_req > 1) {
+      if (tid < TILE_SEGS) sh.pre[tid] = a.hi;
+      __syncthreads();
+      if (tid < c.n_req) {
+        place = 0;
+        for (int r = 0; r < c.n_req; r++) place += sh.pre[r] < a.hi || (sh.pre[r] == a.hi && r < tid);
+      }
     }
+    if (tid < c.n_req) {
+      sh.t0[place] = a.t0; sh.n[place] = a.n; sh.hi[place] = a.hi; sh.r[place] = (unsigned char)tid;
+    }
+    __syncthreads();
+    if (tid < c.n_req) sum = pairs_of(sh.n[tid]);
+  }
+  if (tid < TILE_SEGS) {
     pre = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -277,7 +296,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     for (int step = TILE_SEGS / 2; step; step >>= 1)
       if (sh.pre[lo + step] <= p) lo += step;
     p -= sh.pre[lo];
-    it.r = lo;
+    it.r = sh.r[lo];
     int n_tok = sh.n[lo];
     it.t0 = sh.t0[lo];
     it.end = sh.hi[lo];

@@ -165,8 +165,9 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanCall c) {
 
 // ---------------------------------------------------------------- append ---
 // pool[slot / P][head][slot % P][:] = round(x[token][head][:]), for keys and
-// values.  A thread moves 8 values (16 bytes of cache) of both; bounded by
-// the bytes read and written.
+// values.  A thread has a fixed place of 8 values (16 bytes of cache) in a
+// token's row and moves it for APP_UNROLL tokens at a time, all loads first;
+// bounded by the bytes read and written.
 constexpr int APP_THREADS = 256, APP_UNROLL = 4;
 
 struct AppendCall {
@@ -176,9 +177,10 @@ struct AppendCall {
   int *status;
   long long k_st, k_sh, v_st, v_sh;
   long long kp_st[3], vp_st[3];
-  long long n_vec;          // tokens * heads * dim / 8
   long long n_slots;
-  int page, row_vec, head_vec;   // vectors of a token, of a head
+  int n_tokens, page;
+  int row_vec, head_vec;    // vectors of 8 values in a token, in a head
+  int side;                 // tokens that a block's threads stand side by side for
 };
 
 template <bool F16, bool SRC32>
@@ -196,33 +198,38 @@ QTB_DEV uint4 load8(const void *base, long long at) {
 
 template <bool F16, bool SRC32>
 __global__ void __launch_bounds__(APP_THREADS) append_kernel(const AppendCall c) {
-  const long long step = (long long)gridDim.x * APP_THREADS;
+  const int beside = c.side > 1 ? threadIdx.x / c.row_vec : 0;
+  if (beside >= c.side) return;
   int bad = 0;
-  for (long long i0 = (long long)blockIdx.x * APP_THREADS + threadIdx.x; i0 < c.n_vec; i0 += step * APP_UNROLL) {
-    uint4 kx[APP_UNROLL], vx[APP_UNROLL];
-    long long kd[APP_UNROLL], vd[APP_UNROLL];
+  for (int vec = threadIdx.x - beside * c.row_vec; vec < c.row_vec; vec += APP_THREADS) {
+    const int h = vec / c.head_vec, d = (vec - h * c.head_vec) * 8;
+    const long long ks = h * c.k_sh + d, vs = h * c.v_sh + d, kp = h * c.kp_st[1] + d, vp = h * c.vp_st[1] + d;
+    const int step = gridDim.x * c.side;
+    for (int t0 = blockIdx.x * c.side + beside; t0 < c.n_tokens; t0 += step * APP_UNROLL) {
+      long long s[APP_UNROLL];
+      uint4 kx[APP_UNROLL], vx[APP_UNROLL];
 #pragma unroll
-    for (int u = 0; u < APP_UNROLL; u++) {
-      const long long i = i0 + u * step;
-      kd[u] = -1;
-      if (i >= c.n_vec) continue;
-      const long long t = i / c.row_vec;
-      const int rest = (int)(i - t * c.row_vec), h = rest / c.head_vec, d = (rest - h * c.head_vec) * 8;
-      const long long s = c.slot[t];
-      if (s >= c.n_slots) bad |= QTB_PS_PAGE;
-      if (s < 0 || s >= c.n_slots) continue;
-      const long long pg = s / c.page, off = s - pg * c.page;
-      kx[u] = load8<F16, SRC32>(c.k, t * c.k_st + h * c.k_sh + d);
-      vx[u] = load8<F16, SRC32>(c.v, t * c.v_st + h * c.v_sh + d);
-      kd[u] = pg * c.kp_st[0] + h * c.kp_st[1] + off * c.kp_st[2] + d;
-      vd[u] = pg * c.vp_st[0] + h * c.vp_st[1] + off * c.vp_st[2] + d;
-    }
-#pragma unroll
-    for (int u = 0; u < APP_UNROLL; u++)
-      if (kd[u] >= 0) {
-        *reinterpret_cast<uint4 *>(c.kpool + kd[u]) = kx[u];
-        *reinterpret_cast<uint4 *>(c.vpool + vd[u]) = vx[u];
+      for (int u = 0; u < APP_UNROLL; u++) {
+        const long long t = t0 + (long long)u * step;
+        s[u] = t < c.n_tokens ? c.slot[t] : -1;
+        if (s[u] >= c.n_slots) { bad |= QTB_PS_PAGE; s[u] = -1; }
       }
+#pragma unroll
+      for (int u = 0; u < APP_UNROLL; u++) {
+        if (s[u] < 0) continue;
+        const long long t = t0 + (long long)u * step;
+        kx[u] = load8<F16, SRC32>(c.k, t * c.k_st + ks);
+        vx[u] = load8<F16, SRC32>(c.v, t * c.v_st + vs);
+      }
+#pragma unroll
+      for (int u = 0; u < APP_UNROLL; u++) {
+        if (s[u] < 0) continue;
+        const long long pg = c.n_slots <= 0x7fffffffll ? (long long)((unsigned)s[u] / (unsigned)c.page) : s[u] / c.page;
+        const long long off = s[u] - pg * c.page;
+        *reinterpret_cast<uint4 *>(c.kpool + pg * c.kp_st[0] + off * c.kp_st[2] + kp) = kx[u];
+        *reinterpret_cast<uint4 *>(c.vpool + pg * c.vp_st[0] + off * c.vp_st[2] + vp) = vx[u];
+      }
+    }
   }
   raise_status(c.status, bad);
 }
@@ -414,7 +421,7 @@ extern "C" int qtb_paged_append(const qtb_paged_append_t *d, void *stream) {
   const bool src32 = d->src_dtype == QTB_T_F32;
   if ((d->dtype != QTB_T_BF16 && d->dtype != QTB_T_F16) || (!src32 && d->src_dtype != d->dtype))
     return qtb_fail(QTB_E_UNSUPPORTED, "type %lld into a cache of type %lld: bf16 or f16 from the same or from f32", (long long)d->src_dtype, (long long)d->dtype);
-  if (d->n_tokens < 0 || d->n_tokens >= (1ll << 31) || d->n_kv < 1 || d->n_kv > 1024 || d->head_dim < 8 || d->head_dim % 8 || d->head_dim > 1024)
+  if (d->n_tokens < 0 || d->n_tokens >= (1ll << 30) || d->n_kv < 1 || d->n_kv > 1024 || d->head_dim < 8 || d->head_dim % 8 || d->head_dim > 1024)
     return qtb_fail(QTB_E_INVALID, "%lld tokens, %lld heads of %lld (a multiple of 8)", (long long)d->n_tokens, (long long)d->n_kv, (long long)d->head_dim);
   if (d->page < 1 || d->page > 65536 || d->n_pages < 0 || d->n_pages > INT_MAX)
     return qtb_fail(QTB_E_INVALID, "%lld pages of %lld", (long long)d->n_pages, (long long)d->page);
@@ -433,10 +440,12 @@ extern "C" int qtb_paged_append(const qtb_paged_append_t *d, void *stream) {
   for (int i = 0; i < 3; i++) { c.kp_st[i] = d->kpool_stride[i]; c.vp_st[i] = d->vpool_stride[i]; }
   c.head_vec = (int)d->head_dim / 8;
   c.row_vec = (int)d->n_kv * c.head_vec;
-  c.n_vec = d->n_tokens * c.row_vec;
+  c.n_tokens = (int)d->n_tokens;
+  c.side = c.row_vec < APP_THREADS ? APP_THREADS / c.row_vec : 1;
   c.n_slots = d->n_pages * d->page;
   c.page = (int)d->page;
-  const long long want = (c.n_vec + APP_THREADS - 1) / APP_THREADS;
+  // as many blocks as tokens side by side, up to eight to an SM
+  const long long want = (d->n_tokens + c.side - 1) / c.side;
   const int grid = (int)(want < dev->sms * 8ll ? want : dev->sms * 8ll);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == QTB_T_F16;
