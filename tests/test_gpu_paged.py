@@ -526,3 +526,16 @@ def test_tensors_are_checked(torch, P):
         P.plan(cu, cu[:1], torch.zeros(2, 2, **i32), cu, 16, 4)
     with pytest.raises(ValueError):
         P.plan(cu, cu, torch.zeros(2, 4, **i32)[:, ::2], cu, 16, 4)
+
+
+# -------------------------------------------------------------- all together --
+@pytest.mark.parametrize("rows,chunk,page,name", [(4, 256, 16, "bf16"), (2, 37, 48, "f16")])
+def test_requests_served_in_chunks_equal_whole_prompts(torch, P, rows, chunk, page, name):
+    """Plan, append and paged attention together, pages recycled between requests, against the prompt form.  Both round
+    p and the output, each by at most u of the largest value: twice 2 u between them."""
+    import qtb_paged_step
+    lengths, prompts = [300, 64, 1, 333, 600, 90, 17], [250, 64, 1, 300, 590, 30, 1]
+    worst = qtb_paged_step.serve(lengths, prompts, rows, chunk, page=page, dtype=kind(torch, name))
+    for w in worst:
+        for x in w:
+            assert float(x) <= 4 * U[name], float(x)
