@@ -50,15 +50,14 @@ struct RowsCursor {
   int r, rg, h, ch;      // request, row group, key head, chunk within the item
   int groups, chunks, c0;
 
-  QTB_DEV void load(const AttnCall &c, int row_limit) {   // the request's counts
+  QTB_DEV void load(const AttnCall &c) {   // the request's counts
     a = attn_request<PAGED>(c, r);
-    const int rows = a.n * c.group;
-    groups = rows > row_limit ? 0 : (rows + ROWS_M - 1) / ROWS_M;
+    groups = (a.n * c.group + ROWS_M - 1) / ROWS_M;
     c0 = a.lo / ROWS_CHUNK;
     chunks = max((a.hi + ROWS_CHUNK - 1) / ROWS_CHUNK - c0, 1);
   }
   QTB_DEV long long units(const AttnCall &c) const { return (long long)groups * c.n_kv * chunks; }
-  QTB_DEV void next(const AttnCall &c, int row_limit) {
+  QTB_DEV void next(const AttnCall &c) {
     if (++ch < chunks) return;
     ch = 0;
     if (++h < c.n_kv) return;
@@ -68,7 +67,7 @@ struct RowsCursor {
     do {
       r++;
       if (r >= c.n_req) { groups = 1; chunks = 1; return; }   // past the end: never served
-      load(c, row_limit);
+      load(c);
     } while (groups == 0);
   }
 };
@@ -82,7 +81,7 @@ struct RowsShared {
 
 template <int HD, bool F16, bool PAGED>
 __global__ void __launch_bounds__(ROWS_THREADS, ROWS_PER_SM)
-rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_limit, int box, float *__restrict__ parts,
+rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int box, float *__restrict__ parts,
             AttnCut *__restrict__ cuts) {
   constexpr int KS = HD / 16;              // k-steps of Q K^T
   constexpr int NT = HD / 8;               // 8-wide output tiles
@@ -106,7 +105,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
   const int ra = (int)((long long)c.n_req * tid / ROWS_THREADS), rb = (int)((long long)c.n_req * (tid + 1) / ROWS_THREADS);
   long long sum = 0;
   for (cur.r = ra; cur.r < rb; cur.r++) {
-    cur.load(c, row_limit);
+    cur.load(c);
     sum += cur.units(c);
   }
   long long pre = sum;
@@ -131,7 +130,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
   if (u0 >= pre && u0 < pre + sum) {
     long long at = pre;
     for (cur.r = ra; cur.r < rb; cur.r++) {
-      cur.load(c, row_limit);
+      cur.load(c);
       const long long n = cur.units(c);
       if (u0 < at + n) break;
       at += n;
@@ -141,7 +140,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
   }
   __syncthreads();
   cur.r = sh.req;
-  cur.load(c, row_limit);
+  cur.load(c);
   {
     unsigned long long off = (unsigned long long)sh.off;
     cur.ch = (int)(off % (unsigned)cur.chunks);
@@ -199,7 +198,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
         if (PAGED && (pg < 0 || pg >= c.n_pages)) { pg = c.n_pages; bad = QTB_PS_PAGE; }   // past the last page: zeros
         tma_load_5d(dst0 + st * 2 * KEYS_B, map, 0, off, 0, cur.h, PAGED ? pg : 0, &sh.full[st]);
       }
-      cur.next(c, row_limit);
+      cur.next(c);
       if (u + 1 < n_units) find();
     }
     // copies in flight land before the block leaves
@@ -401,7 +400,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int row_lim
       fresh = true;
       starts = true;
     }
-    cur.next(c, row_limit);
+    cur.next(c);
   }
 }
 
@@ -429,41 +428,40 @@ static inline bool rows_maps(const AttnCall &c, bool paged, bool f16, int hd, Te
 }
 
 template <int HD, bool F16, bool PAGED>
-static cudaError_t rows_run(bool prepare, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, int max_rows, void *ws,
+static cudaError_t rows_run(bool prepare, const AttnCall *c, const RowsMaps *m, int sms, int max_rows, void *ws,
                             cudaStream_t st) {
   if (prepare)
     return cudaFuncSetAttribute(rows_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, rows_smem<HD>());
   const int grid = sms * ROWS_PER_SM;
   AttnCut *cuts = static_cast<AttnCut *>(ws);
   float *parts = reinterpret_cast<float *>(cuts + grid);
-  rows_kernel<HD, F16, PAGED><<<grid, ROWS_THREADS, rows_smem<HD>(), st>>>(*c, *m, row_limit, rows_box(PAGED, c->page), parts, cuts);
+  rows_kernel<HD, F16, PAGED><<<grid, ROWS_THREADS, rows_smem<HD>(), st>>>(*c, *m, rows_box(PAGED, c->page), parts, cuts);
   if (cudaError_t e = cudaGetLastError()) return e;
   return launch_early(join_kernel<HD, F16, ROWS_M, 1, JOIN_WARPS, 1>, dim3(grid, max_rows), 32 * JOIN_WARPS, 0, st, *c, (const float *)parts,
                       (const AttnCut *)cuts);
 }
-// Requests with at most row_limit query rows to a key head are served; max_rows
-// is how many rows (of 16) an item may have, as far as known.
-static inline cudaError_t rows_any(bool prepare, int which, const AttnCall *c, const RowsMaps *m, int sms, int row_limit, int max_rows,
+// max_rows: how many rows (of 16) an item has, as far as known.
+static inline cudaError_t rows_any(bool prepare, int which, const AttnCall *c, const RowsMaps *m, int sms, int max_rows,
                                    void *ws, cudaStream_t st) {
   switch (which) {
-    case 0: return rows_run<64, false, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    case 1: return rows_run<64, false, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    case 2: return rows_run<64, true, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    case 3: return rows_run<64, true, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    case 4: return rows_run<128, false, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    case 5: return rows_run<128, false, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    case 6: return rows_run<128, true, false>(prepare, c, m, sms, row_limit, max_rows, ws, st);
-    default: return rows_run<128, true, true>(prepare, c, m, sms, row_limit, max_rows, ws, st);
+    case 0: return rows_run<64, false, false>(prepare, c, m, sms, max_rows, ws, st);
+    case 1: return rows_run<64, false, true>(prepare, c, m, sms, max_rows, ws, st);
+    case 2: return rows_run<64, true, false>(prepare, c, m, sms, max_rows, ws, st);
+    case 3: return rows_run<64, true, true>(prepare, c, m, sms, max_rows, ws, st);
+    case 4: return rows_run<128, false, false>(prepare, c, m, sms, max_rows, ws, st);
+    case 5: return rows_run<128, false, true>(prepare, c, m, sms, max_rows, ws, st);
+    case 6: return rows_run<128, true, false>(prepare, c, m, sms, max_rows, ws, st);
+    default: return rows_run<128, true, true>(prepare, c, m, sms, max_rows, ws, st);
   }
 }
 static inline cudaError_t rows_prepare() {
   for (int i = 0; i < 8; i++)
-    if (cudaError_t e = rows_any(true, i, nullptr, nullptr, 0, 0, 0, nullptr, nullptr)) return e;
+    if (cudaError_t e = rows_any(true, i, nullptr, nullptr, 0, 0, nullptr, nullptr)) return e;
   return cudaSuccess;
 }
-static inline cudaError_t rows_launch(const AttnCall &c, bool paged, bool f16, int hd, const RowsMaps &m, int sms, int row_limit,
-                                      int max_rows, void *ws, cudaStream_t st) {
-  return rows_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, row_limit, max_rows, ws, st);
+static inline cudaError_t rows_launch(const AttnCall &c, bool paged, bool f16, int hd, const RowsMaps &m, int sms, int max_rows,
+                                       void *ws, cudaStream_t st) {
+  return rows_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, max_rows, ws, st);
 }
 
 }  // namespace qtb

@@ -208,7 +208,7 @@ struct TileItem {
 
 template <int HD, bool F16, bool PAGED>
 __global__ void __launch_bounds__(TILE_THREADS, 1)
-tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_limit, int tpt, int box,
+tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, int box,
             float *__restrict__ parts, AttnCut *__restrict__ cuts) {
   constexpr int STAGES = tile_stages<HD>(), KV_B = tile_kv_bytes<HD>(), Q_B = TILE_M * HD * 2, HALF_B = TILE_M * 128;
   constexpr uint32_t S_COL = 0, O_COL = 256;
@@ -237,10 +237,9 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int row_lim
     sy.abort = 0;
     fence_mbar_init();
   }
-  // --- pairs of every request (those with more than row_limit rows), summed over
-  // runs of requests: one of the first 128 threads has a run
+  // --- pairs of every request, summed over runs of requests: one of the first 128 threads has a run
   const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS;
-  auto pairs_of = [&](int n) { return n * c.group > row_limit ? (n + 2 * tpt - 1) / (2 * tpt) : 0; };
+  auto pairs_of = [&](int n) { return (n + 2 * tpt - 1) / (2 * tpt); };
   int sum = 0, pre = 0;
   if (seg > 1) {
     if (tid < TILE_SEGS)
@@ -844,45 +843,44 @@ static inline size_t tile_workspace(int hd, int sms) {
 }
 
 template <int HD, bool F16, bool PAGED>
-static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, int sms, int row_limit, void *ws, cudaStream_t st) {
+static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, int sms, void *ws, cudaStream_t st) {
   if (prepare)
     return cudaFuncSetAttribute(tile_kernel<HD, F16, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_smem<HD>());
   const int tpt = TILE_M / c->group, box = tile_box(PAGED, c->page);
   if (!ws) {                               // whole items only
     const long long items = ((c->n_tokens + 2 * tpt - 1) / (2 * tpt) + (c->n_req > 1 ? c->n_req : 0)) * (long long)c->n_kv;   // at most
-    tile_kernel<HD, F16, PAGED><<<(int)(items < sms ? items : sms), TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tpt, box, nullptr, nullptr);
+    tile_kernel<HD, F16, PAGED><<<(int)(items < sms ? items : sms), TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, tpt, box, nullptr, nullptr);
     return cudaGetLastError();
   }
   AttnCut *cuts = static_cast<AttnCut *>(ws);
   float *parts = reinterpret_cast<float *>(cuts + sms);
-  tile_kernel<HD, F16, PAGED><<<sms, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, row_limit, tpt, box, parts, cuts);
+  tile_kernel<HD, F16, PAGED><<<sms, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, tpt, box, parts, cuts);
   if (cudaError_t e = cudaGetLastError()) return e;
   return launch_early(join_kernel<HD, F16, TILE_M, 2, 1, 4>, dim3(sms, 2 * TILE_M / (4 * JOIN_WARPS)), 32 * JOIN_WARPS, 0, st, *c,
                       (const float *)parts, (const AttnCut *)cuts);
 }
-static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int sms, int row_limit, void *ws,
+static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int sms, void *ws,
                                    cudaStream_t st) {
   switch (which) {
-    case 0: return tile_run<64, false, false>(prepare, c, m, sms, row_limit, ws, st);
-    case 1: return tile_run<64, false, true>(prepare, c, m, sms, row_limit, ws, st);
-    case 2: return tile_run<64, true, false>(prepare, c, m, sms, row_limit, ws, st);
-    case 3: return tile_run<64, true, true>(prepare, c, m, sms, row_limit, ws, st);
-    case 4: return tile_run<128, false, false>(prepare, c, m, sms, row_limit, ws, st);
-    case 5: return tile_run<128, false, true>(prepare, c, m, sms, row_limit, ws, st);
-    case 6: return tile_run<128, true, false>(prepare, c, m, sms, row_limit, ws, st);
-    default: return tile_run<128, true, true>(prepare, c, m, sms, row_limit, ws, st);
+    case 0: return tile_run<64, false, false>(prepare, c, m, sms, ws, st);
+    case 1: return tile_run<64, false, true>(prepare, c, m, sms, ws, st);
+    case 2: return tile_run<64, true, false>(prepare, c, m, sms, ws, st);
+    case 3: return tile_run<64, true, true>(prepare, c, m, sms, ws, st);
+    case 4: return tile_run<128, false, false>(prepare, c, m, sms, ws, st);
+    case 5: return tile_run<128, false, true>(prepare, c, m, sms, ws, st);
+    case 6: return tile_run<128, true, false>(prepare, c, m, sms, ws, st);
+    default: return tile_run<128, true, true>(prepare, c, m, sms, ws, st);
   }
 }
 static inline cudaError_t tile_prepare() {
   for (int i = 0; i < 8; i++)
-    if (cudaError_t e = tile_any(true, i, nullptr, nullptr, 0, 0, nullptr, nullptr)) return e;
+    if (cudaError_t e = tile_any(true, i, nullptr, nullptr, 0, nullptr, nullptr)) return e;
   return cudaSuccess;
 }
-// Requests with more than row_limit query rows to a key head are served; without
-// a workspace no item is cut.
-static inline cudaError_t tile_launch(const AttnCall &c, bool paged, bool f16, int hd, const TileMaps &m, int sms, int row_limit,
-                                      void *ws, cudaStream_t st) {
-  return tile_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, row_limit, ws, st);
+// Without a workspace no item is cut.
+static inline cudaError_t tile_launch(const AttnCall &c, bool paged, bool f16, int hd, const TileMaps &m, int sms, void *ws,
+                                       cudaStream_t st) {
+  return tile_any(false, (hd == 128 ? 4 : 0) + (f16 ? 2 : 0) + (paged ? 1 : 0), &c, &m, sms, ws, st);
 }
 
 }  // namespace qtb

@@ -334,30 +334,25 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
   return QTB_OK;
 }
 
-// Which kernel has a request goes by its query rows to a key head: few rows over
-// a long cache want the split key axis of the rows kernel, many rows the tiles;
-// prompts have no long cache.  max_new, where it is given, saves a launch.
+// Which kernel has the call.  The rows kernel, where every request has few query
+// rows to a key head, as max_new tells (and in the forms that the tile kernel does
+// not read); the tile kernel, where any has many, and for prompts, which have no
+// long cache to split.  A mixed call goes to the tiles as a whole: single tokens
+// fill them badly, but their keys stream at the same rate, and a second pair of
+// launches costs more (us, tiles / rows and tiles: 16 requests of up to 7000 keys,
+// every fourth with 400 new tokens, 222 / 236; 64 of 1000, every fourth with 64,
+// 71 / 74; 4 of 500, one with 64, 17 / 26).
 struct AttnPlan {
-  bool rows, tiles;
-  int limit;               // rows kernel: requests of at most so many rows
-  bool cut;                // tiles: items may be cut between blocks
-  size_t rows_ws, ws;      // bytes: the rows kernel's workspace, then the tiles'
+  bool tiles;
+  bool cut;                // items may be cut between blocks
+  size_t ws;               // bytes of workspace
 };
 AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged, int sms) {
   AttnPlan p;
-  p.tiles = tile_form(c);
-  p.limit = !p.tiles ? INT_MAX : paged ? ROWS_M : 0;
-  if (p.tiles && paged && d->max_new > 0 && d->max_new * c.group <= ROWS_M) {
-    p.tiles = false;
-    p.limit = INT_MAX;
-  }
-  // one request, or all alike: none has few rows beside many
-  if (p.tiles && (c.n_req == 1 || d->max_new * c.n_req == d->n_tokens) && c.n_tokens / c.n_req * c.group > ROWS_M) p.limit = 0;
-  p.rows = p.limit > 0;
+  p.tiles = tile_form(c) && !(paged && d->max_new > 0 && d->max_new * c.group <= ROWS_M);
   // a few key tiles are not worth a second launch
   p.cut = p.tiles && !(d->max_kv > 0 && d->max_kv <= 4 * TILE_N);
-  p.rows_ws = p.rows ? rows_workspace((int)d->head_dim, sms) : 0;
-  p.ws = p.rows_ws + (p.cut ? tile_workspace((int)d->head_dim, sms) : 0);
+  p.ws = !p.tiles ? rows_workspace((int)d->head_dim, sms) : p.cut ? tile_workspace((int)d->head_dim, sms) : 0;
   return p;
 }
 
@@ -376,14 +371,17 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = d->dtype == QTB_T_F16;
   const int hd = (int)d->head_dim;
-  TileMaps tm;
-  RowsMaps rm;
-  if ((p.tiles && !tile_maps(c, paged, f16, hd, dev->encode, tm)) || (p.rows && !rows_maps(c, paged, f16, hd, dev->encode, rm)))
-    return qtb_fail(QTB_E_UNSUPPORTED, "q, k or v have strides or extents that a tensor map cannot hold");
-  char *ws = static_cast<char *>(d->workspace);
-  const int max_rows = d->max_new > 0 && d->max_new * c.group < ROWS_M ? (int)d->max_new * c.group : ROWS_M;
-  if (p.rows) PAGED_TRY(rows_launch(c, paged, f16, hd, rm, dev->sms, p.limit, max_rows, ws, st));
-  if (p.tiles) PAGED_TRY(tile_launch(c, paged, f16, hd, tm, dev->sms, p.limit, p.cut ? ws + p.rows_ws : nullptr, st));
+  static const char *const no_map = "q, k or v have strides or extents that a tensor map cannot hold";
+  if (p.tiles) {
+    TileMaps m;
+    if (!tile_maps(c, paged, f16, hd, dev->encode, m)) return qtb_fail(QTB_E_UNSUPPORTED, no_map);
+    PAGED_TRY(tile_launch(c, paged, f16, hd, m, dev->sms, p.cut ? d->workspace : nullptr, st));
+  } else {
+    RowsMaps m;
+    const int max_rows = d->max_new > 0 && d->max_new * c.group < ROWS_M ? (int)d->max_new * c.group : ROWS_M;
+    if (!rows_maps(c, paged, f16, hd, dev->encode, m)) return qtb_fail(QTB_E_UNSUPPORTED, no_map);
+    PAGED_TRY(rows_launch(c, paged, f16, hd, m, dev->sms, max_rows, d->workspace, st));
+  }
   return QTB_OK;
 }
 
