@@ -37,8 +37,9 @@
 //
 // Products are issued in order, so the commit that completes S of tile j also
 // says that P V of tile j - 1 is in O: the softmax warps may scale O then.
-// Every wait is bounded; one that runs out raises QTB_PS_TIMEOUT and all roles
-// leave.
+// Every wait is bounded; one that runs out raises QTB_PS_TIMEOUT, and the roles
+// run on to their end without waiting (what they then read and write lies within
+// the block's own buffers and outputs).
 #pragma once
 #include "qtb_paged.cuh"
 
@@ -149,17 +150,37 @@ template <int N>
 QTB_DEV void regs_take() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 QTB_DEV void regs_give() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
-// Whether the phase has completed, after waiting a short while for it.
-QTB_DEV bool mbar_try(uint64_t *bar, uint32_t parity) {
+// Waits for a phase, for a bounded number of the hardware's suspensions; 0 where it
+// has not completed.  (The loop is written out: the MMA warp's reaction to a
+// barrier is on the path between two tiles.)
+QTB_DEV uint32_t mbar_tries(uint32_t bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t.reg .u32 n;\n\t"
+      "mov.u32 n, 1024;\n\t"
+      "MBAR_TRY:\n\t"
       "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "@p bra MBAR_DONE;\n\t"
+      "sub.u32 n, n, 1;\n\t"
+      "setp.ne.u32 q, n, 0;\n\t"
+      "@q bra MBAR_TRY;\n\t"
+      "MBAR_DONE:\n\t"
       "selp.u32 %0, 1, 0, p;\n\t}"
       : "=r"(done)
-      : "r"(smem_u32(bar)), "r"(parity)
+      : "r"(bar), "r"(parity)
       : "memory");
-  return done != 0;
+  return done;
+}
+QTB_DEV bool tile_wait_long(uint32_t bar, uint32_t parity, volatile int *abort, int *status) {
+  const long long t0 = clock64();
+  while (!*abort) {
+    if (mbar_tries(bar, parity)) return true;
+    if (clock64() - t0 > TILE_WAIT) {
+      *abort = 1;
+      raise_status(status, QTB_PS_TIMEOUT);
+    }
+  }
+  return false;
 }
 // True in one lane of the (converged) warp, always the same one.
 QTB_DEV bool elect_one() {
@@ -422,21 +443,13 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     it.n1 = max(min(to, it.n1), from);
     return true;
   };
-  // Bounded wait of a whole warp; false: this or another role gave up.
+  // Bounded wait of a whole warp; false: it, or another role's, ran out.
   auto wait = [&](uint64_t *bar, uint32_t parity) {
-    bool ok = mbar_try(bar, parity);
-    if (!ok) {
-      const long long t0 = clock64();
-      for (int n = 0; !(ok = mbar_try(bar, parity)); n++) {
-        if ((n & 15) != 15) continue;
-        if (*reinterpret_cast<volatile int *>(&sy.abort)) break;
-        if (clock64() - t0 > TILE_WAIT) {
-          *reinterpret_cast<volatile int *>(&sy.abort) = 1;
-          raise_status(c.status, QTB_PS_TIMEOUT);
-        }
-      }
-    }
-    return (bool)__all_sync(0xffffffffu, ok);
+    const uint32_t at = smem_u32(bar);
+    bool ok = true;
+    if (!mbar_tries(at, parity)) ok = tile_wait_long(at, parity, &sy.abort, c.status);
+    __syncwarp();
+    return ok;
   };
 
   if (warp >= 8) {
@@ -453,7 +466,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       const int to = max(it.n0, it.n1);
       if (to == it.from) continue;
       auto load_q = [&]() {
-        if (!wait(&sy.q_empty, (n_items & 1) ^ 1)) return false;
+        if (!__all_sync(0xffffffffu, wait(&sy.q_empty, (n_items & 1) ^ 1))) return false;
         if (lane == 0) {
           const int rows = tpt * c.group, two = it.tok1 > 0;
           mbar_arrive_expect_tx(&sy.q_full, (uint32_t)(rows * 128 * (HD / 64) * (1 + two)));
@@ -482,7 +495,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
 #pragma unroll
         for (int kv = 0; kv < 2; kv++) {
           const int st = (int)(fill % STAGES);
-          if (!wait(&sy.kv_empty[st], ((fill / STAGES) & 1) ^ 1)) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, wait(&sy.kv_empty[st], ((fill / STAGES) & 1) ^ 1))) { ok = false; break; }
           if (lane == 0) mbar_arrive_expect_tx(&sy.kv_full[st], (uint32_t)(count * box * 128));
           __syncwarp();
           if (mine) {
@@ -508,17 +521,17 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     const uint32_t idesc_s = umma_idesc(1u, ab, TILE_N), idesc_o = umma_idesc(1u, ab, HD) | (1u << 16);   // B as [K][N]
     uint32_t fill = 0, n_items = 0;
     uint32_t p_n = 0, o_n = 0;             // bit t: parity of the P hand-overs, of the finished outputs of tile t
-    bool ok = true, issued = false;
+    bool issued = false;
     // descriptors of the first tile and stage: others are an address (in 16 bytes) further on
     const uint64_t q_desc = umma_desc_sw128(smem_u32(s_q)), k_desc = umma_desc_sw128(smem_u32(s_kv));
     const uint64_t v_desc = umma_desc_mn128(smem_u32(s_kv), HALF_B);
 #pragma unroll 1
-    for (int i = 0; ok; i++) {
+    for (int i = 0;; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
       const int to = max(it.n0, it.n1);
       if (to == it.from) continue;
-      if (!wait(&sy.q_full, n_items & 1)) break;
+      wait(&sy.q_full, n_items & 1);
       n_items++;
       auto scores = [&](int t, int st) {
         const uint64_t q = q_desc + (uint32_t)(t * (Q_B >> 4)), k = k_desc + (uint32_t)(st * (KV_B >> 4));
@@ -534,7 +547,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         __syncwarp();
       };
       int st = (int)(fill % STAGES);
-      if (!(ok = wait(&sy.kv_full[st], (fill / STAGES) & 1))) break;
+      wait(&sy.kv_full[st], (fill / STAGES) & 1);
       issued = true;
       if (it.n0 > it.from) scores(0, st);
       if (it.n1 > it.from) scores(1, st);
@@ -545,7 +558,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       __syncwarp();
       fill++;
 #pragma unroll 1
-      for (int j = it.from; j < to && ok; j++) {
+      for (int j = it.from; j < to; j++) {
         const int sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
         const bool more = j + 1 < to;
 #pragma unroll
@@ -559,7 +572,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
           if (lane == 1) { bar = &sy.kv_full[sv]; par = (fill / STAGES) & 1; }
           if (lane == 2 && more) { bar = &sy.kv_full[sk]; par = ((fill + 1) / STAGES) & 1; }
           if (lane == 3 && j == it.from) { bar = &sy.o_empty[t]; par = ((o_n >> t) & 1) ^ 1; }
-          if (!(ok = wait(bar, par))) break;
+          wait(bar, par);
           tc_fence_after();
           const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
           const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
@@ -568,7 +581,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
             for (int ks = 0; ks < TILE_N / 32; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, j > it.from || ks > 0);
           }
           __syncwarp();
-          if (!(ok = wait(&sy.p_full[t][1], (p_n >> t) & 1))) break;
+          wait(&sy.p_full[t][1], (p_n >> t) & 1);
           p_n ^= 1u << t;
           tc_fence_after();
           if (elect_one()) {
@@ -580,7 +593,6 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
           if (j == n - 1) o_n ^= 1u << t;
           if (j + 1 < n) scores(t, sk);
         }
-        if (!ok) break;
         if (elect_one()) {
           umma_commit(&sy.kv_empty[sv]);
           if (more) umma_commit(&sy.kv_empty[sk]);
@@ -618,10 +630,9 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       const int clear_a = c.window > 0 ? (max(pos_b - c.window + 1, 0) - it.k0 + TILE_N - 1) / TILE_N : 0;
       const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
       float m = -INFINITY, l = 0.f;
-      bool ok = true;
 #pragma unroll 1
       for (int j = it.from; j < n; j++) {
-        if (!(ok = wait(&sy.s_full[t], s_n & 1))) break;
+        wait(&sy.s_full[t], s_n & 1);
         s_n++;
         tc_fence_after();
         float s[128];
@@ -645,7 +656,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
             // keys that no row sees: their V may be anything, and 0 * NaN is NaN
             const uint32_t f = fill + 2 * (j - it.from) + 1;
             unsigned char *v = s_kv + (f % STAGES) * KV_B;
-            if (!(ok = wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1))) break;
+            wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1);
             if (kb + row < it.low || kb + row >= it.high) {
 #pragma unroll 1
               for (int y = 0; y < 8 * (HD / 64); y++)
@@ -733,11 +744,10 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         f2_get(add2(sum[0], sum[1]), la, lb);
         l += la + lb;
       }
-      if (!ok) break;
       fill += 2 * (to - it.from);
       const bool some = n > it.from;
       if (some) {
-        if (!wait(&sy.o_full[t], o_n & 1)) break;
+        wait(&sy.o_full[t], o_n & 1);
         o_n++;
         tc_fence_after();
       }
