@@ -48,8 +48,13 @@ namespace qtb {
 constexpr int TILE_THREADS = 384, TILE_M = 128, TILE_N = 128;
 // Registers of a thread: the block starts with 168 for each of its 384 threads
 // (64512 in all); the softmax warps, a row of S each, take what the loading and
-// issuing warpgroup gives up: 256 * 200 + 128 * 96 = 63488.
-constexpr int TILE_REGS_SOFTMAX = 200, TILE_REGS_OTHER = 96;
+// issuing warpgroup gives up: 256 * 208 + 128 * 80 = 256 * 200 + 128 * 96 = 63488.
+// (16384-token prompt of 128 dims 845 us with 208, 859 with 200; 8192 tokens of 64
+// dims 192 and 185.)
+template <int HD>
+constexpr int tile_regs_softmax() { return HD == 128 ? 208 : 200; }
+template <int HD>
+constexpr int tile_regs_other() { return HD == 128 ? 80 : 96; }
 constexpr int TILE_CUT = 1;                // key tiles that a block has of an item at least, where it has not all
 constexpr int TILE_SEGS = 128;             // runs of requests that the in-block search tells apart
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
@@ -75,6 +80,11 @@ struct TileSync {
   uint32_t tmem;
   int abort;
 };
+
+// Whether `items` fill `grid` blocks evenly enough to be dealt out whole.
+QTB_HOST_DEV bool tile_whole(long long items, int grid) {
+  return 2 * items >= 5 * grid || (items <= grid && 4 * items >= 3 * grid);
+}
 
 // What lies in shared memory behind the operands (which start it, on 1024 bytes).
 struct TileShared {
@@ -343,7 +353,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   // than TILE_CUT key tiles would be left on that side.
   const int items = pairs * c.n_kv;        // the host has bounded it
   const int grid = (int)gridDim.x;
-  const bool deal = !parts || 2 * (long long)items >= 5 * grid || (items <= grid && 4 * items >= 3 * grid);
+  const bool deal = !parts || tile_whole(items, grid);
   if (deal) {
     if (tid == 0 && parts) cuts[blockIdx.x].last = -1;
   } else {
@@ -453,7 +463,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   };
 
   if (warp >= 8) {
-    regs_give<TILE_REGS_OTHER>();
+    regs_give<tile_regs_other<HD>()>();
     if (warp == 8) {
     // ------------------------------------------------------------- loads ---
     int bad = 0;
@@ -609,7 +619,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     }
     }
   } else {
-    regs_take<TILE_REGS_SOFTMAX>();
+    regs_take<tile_regs_softmax<HD>()>();
     // ----------------------------------------------------------- softmax ---
     const int t = warp >> 2, row = tid & 127;
     const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;

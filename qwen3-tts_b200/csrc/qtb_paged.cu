@@ -350,8 +350,9 @@ struct AttnPlan {
 AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged, int sms) {
   AttnPlan p;
   p.tiles = tile_form(c) && !(paged && d->max_new > 0 && d->max_new * c.group <= ROWS_M);
-  // a few key tiles are not worth a second launch
-  p.cut = p.tiles && !(d->max_kv > 0 && d->max_kv <= 4 * TILE_N);
+  // no second launch for a few key tiles, nor where one request's items are seen to fill the blocks
+  const long long pair = 2 * (TILE_M / c.group), items = (c.n_tokens + pair - 1) / pair * c.n_kv;
+  p.cut = p.tiles && !(d->max_kv > 0 && d->max_kv <= 4 * TILE_N) && !(c.n_req == 1 && tile_whole(items, sms));
   p.ws = !p.tiles ? rows_workspace((int)d->head_dim, sms) : p.cut ? tile_workspace((int)d->head_dim, sms) : 0;
   return p;
 }
