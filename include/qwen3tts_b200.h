@@ -336,16 +336,19 @@ int qtb_attention_noalloc(const float *qkv, int batch, int n_heads, int n_kv, in
  * qtb_paged_plan once, then per layer qtb_paged_append and qtb_paged_attention
  * (or qtb_prompt_attention, when every request starts from nothing and K and V
  * are at hand).  They have no counterpart in the reference, whose cache is one
- * request's contiguous rows.  Every pointer is DEVICE memory of the current
- * device owned by the caller, `stream` a cudaStream_t (NULL = legacy default
- * stream).  A call checks its arguments on the host, launches and returns: it
- * never allocates, synchronises or keeps state, and may be captured into a
- * graph.  Request lengths, page numbers and slots live on the device, so the
- * kernels check them there: what is out of range is not accessed, and the
- * reason is ORed into *status (NULL: not reported), which the caller zeroes.
- * Every field is 64 bits wide; strides are in elements, the innermost
- * dimension is contiguous, no axis is expanded (stride 0), and tensor pointers and strides are multiples of 16
- * bytes.  Nothing is read from tensors of extent zero. */
+ * request's contiguous rows.
+ *
+ * Every pointer is DEVICE memory of the current device, owned by the caller;
+ * `stream` is a cudaStream_t (NULL = legacy default stream).  A call checks its
+ * arguments on the host, launches and returns: it never allocates, synchronises
+ * or keeps state, and may be captured into a graph.  Request lengths, page
+ * numbers and slots live on the device, so the kernels check them there: what
+ * is out of range is not accessed, and the reason is ORed into *status (NULL:
+ * not reported), which the caller zeroes.
+ *
+ * Every field is 64 bits wide.  Strides are in elements; the innermost dimension
+ * is contiguous, no axis of q, k, v or out is expanded (stride 0), and tensor
+ * pointers and strides are multiples of 16 bytes. */
 enum {
     QTB_T_F32 = 0,
     QTB_T_BF16 = 1,
@@ -422,9 +425,10 @@ typedef struct {
     int64_t dtype, causal, window;
     double scale;
 } qtb_attn_t;
-/* Bytes of workspace for a call of the paged or the prompt form with these sizes,
- * strides and scale (addresses matter for their alignment alone), or a negative QTB_E_* code.  Its
- * contents matter during one call only. */
+/* Bytes of workspace for a call of the paged or the prompt form with these
+ * sizes, strides and scale (addresses matter for their alignment alone), or a
+ * negative QTB_E_* code.  Its contents matter during one call only; a call that
+ * is given too little returns QTB_E_WORKSPACE. */
 int64_t qtb_attn_workspace(const qtb_attn_t *d, int paged);
 int qtb_paged_attention(const qtb_attn_t *d, void *stream);
 int qtb_prompt_attention(const qtb_attn_t *d, void *stream);

@@ -19,8 +19,14 @@
 // What bounds it is the stream of K and V.  One warp copies by TMA (a box is a
 // run of a page's positions with all of its dims, 128-byte swizzle), four
 // compute; two blocks of three 64-key stages on an SM keep up to 192 KB in
-// flight.  Keys outside the request may hold anything: their scores become
-// -inf and their V is masked to zero in registers.
+// flight.  (Copies of 16 bytes issued by the computing warps themselves reached
+// half the rate.)  Keys outside the request may hold anything: their scores
+// become -inf and their V is masked to zero in registers.
+//
+// Measured, with the join: 128 requests of 4096 to 16384 keys, 32 / 4 heads, pages
+// of 64: 423 to 430 us, 6.5 TB/s, the rate of a plain copy; 64 requests of 256 to
+// 4096 keys, 16 / 8 heads, pages of 16: 85 us, 5.75 TB/s; one request of 4096
+// keys: 11 us, the latency of two dependent launches.
 #pragma once
 #include "qtb_paged.cuh"
 #include <cuda.h>

@@ -35,6 +35,18 @@
 // prompt, 512 items, 212 / 272; 4 x 512 tokens over 8192 keys, 128 items, 122 /
 // 137; 8 x 64 tokens over 8192 keys, 64 items, 133 / 75).
 //
+// What bounds it.  A step (two query tiles, one key tile) needs 2048 cycles of the
+// tensor pipe at 128 dims and 2048 of the MUFU's exponentials, and takes about
+// 3400: both pipes 60 % busy (8192-token prompt, 16 / 8 heads), with the chain
+// scores - softmax - P V - next scores of one tile under the other's.  Tried and
+// not kept (8192 tokens): a quarter of the exponentials by a polynomial on the FMA
+// pipe (-2 to -4 %), two threads to a row (-18 %), P handed over in one piece
+// (-1 %), in three (-11 %).  Measured: a 16384-token prompt, 16 / 8 heads, 128 dims
+// 820 to 960 us by the clock that the power limit leaves (1150 to 1340 TFLOP/s);
+// 8192 tokens 215 to 225 us, of 64 dims, where the exponentials weigh twice, 186
+// us (740 TFLOP/s).  A short call is its start: 64 tokens take 9 us, of which a
+// launch is 2 and most of the rest code fetched for the first time.
+//
 // Products are issued in order, so the commit that completes S of tile j also
 // says that P V of tile j - 1 is in O: the softmax warps may scale O then.
 // Every wait is bounded; one that runs out raises QTB_PS_TIMEOUT, and the roles

@@ -118,7 +118,9 @@ constexpr int JOIN_WARPS = 8;
 // then part 0 of the following ones.  WPR warps share a row (they take every
 // WPR-th part and join theirs in warp order), or a warp has RPW rows side by
 // side; a lane has HD / 32 dims of each.  Bounded by the latency of a part's
-// loads: those of UNROLL parts of all its rows are in flight together.
+// loads for few parts (those of UNROLL parts of all its rows are in flight
+// together), by their bytes for many: 148 cut items of 256 rows are about 40 MB
+// and 14 us.
 template <int HD, bool F16, int M, int TILES, int WPR, int RPW>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 join_kernel(const AttnCall c, const float *__restrict__ parts, const AttnCut *__restrict__ cuts) {
