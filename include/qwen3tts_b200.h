@@ -406,7 +406,8 @@ int qtb_paged_append(const qtb_paged_append_t *d, void *stream);
  * token at position p sees keys <= p (causal != 0) and > p - window (window >
  * 0).  out = softmax(scale q.k) v in the type of q; lse = log sum exp(scale
  * q.k), natural, f32 [n_tokens][n_heads] (NULL: not wanted).  A token that sees
- * no key gets zeros and -inf.  head_dim 64 or 128; page a multiple of 16.
+ * no key gets zeros and -inf; tokens outside cu_new[0] .. cu_new[n_req] (room
+ * for a larger step) are not written.  head_dim 64 or 128; page a multiple of 16.
  * max_new and max_kv bound new_len and kv_len over the requests: they choose
  * how the work is split, not what is computed (0: not known). */
 typedef struct {

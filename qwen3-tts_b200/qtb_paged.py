@@ -48,6 +48,7 @@ _this_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream   # what torch.cuda.current_stream(i).cuda_stream is, without the object
 
 _NEEDS = -6                 # QTB_E_WORKSPACE
+_sizes = {}                 # bytes of workspace of paged calls by (device, head_dim, few rows?)
 _calls = None
 
 
@@ -169,14 +170,20 @@ def _results(q, out, lse, status, dev):
     return out, lse
 
 
-def _attend(fn, pool, dev, q, head, tail):
-    """One attention call, and the workspace that it says it needs."""
-    rc = _NEEDS if pool else _on_device(dev, fn, _ATTN(*head, 0, 0, *tail), _stream_of(dev))
+def _attend(fn, pool, dev, q, head, tail, few=False):
+    """One attention call with the workspace that calls of its kind have needed so far, and again with what
+    qtb_attn_workspace asks for where that is not enough."""
+    key = (dev, q.shape[2], few) if pool else None
+    size = _sizes.get(key, 0)
+    ws = q.new_empty(size // 2) if size else None          # of two-byte values
+    rc = _on_device(dev, fn, _ATTN(*head, 0 if ws is None else ws.data_ptr(), size, *tail), _stream_of(dev))
     if rc == _NEEDS:
         size = _on_device(dev, _lib().qtb_attn_workspace, _ATTN(*head, 0, 0, *tail), pool)
         if size < 0:
             Q.check(size)
-        ws = q.new_empty(size // 2)              # of two-byte values
+        if pool:
+            _sizes[key] = size
+        ws = q.new_empty(size // 2)
         rc = _on_device(dev, fn, _ATTN(*head, ws.data_ptr(), size, *tail), _stream_of(dev))
     if rc:
         Q.check(rc)
@@ -190,7 +197,8 @@ def paged_attention(q, kpool, vpool, table, cu_new, kv_len, max_new: int = 0, ma
     int32 [requests], cached tokens with the new ones, which are the last.
     window: how many keys a token looks back on, itself included (0: all).
     max_new, max_kv: bounds of new tokens and keys per request, to choose the
-    split of the work (0: not known).  Returns (out, lse)."""
+    split of the work (0: not known).  Returns (out, lse), whose rows past
+    cu_new[-1] are not written."""
     dev = q.get_device()
     t, h, d = q.shape
     pages, kv, page, _ = pools = kpool.shape
@@ -209,7 +217,8 @@ def paged_attention(q, kpool, vpool, table, cu_new, kv_len, max_new: int = 0, ma
             (q.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), out.data_ptr(), lse.data_ptr(), cu_new.data_ptr(), kv_len.data_ptr(),
              table.data_ptr(), 0 if status is None else status.data_ptr()),
             (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.stride(0), cols, page, pages, n, t, h, kv, d,
-             max_new, max_kv, _TYPES[kind], causal, window or 0, 1 / math.sqrt(d) if scale is None else scale))
+             max_new, max_kv, _TYPES[kind], causal, window or 0, 1 / math.sqrt(d) if scale is None else scale),
+            0 < max_new * h <= 16 * kv)
     return out, lse
 
 
