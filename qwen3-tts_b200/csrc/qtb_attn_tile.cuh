@@ -888,7 +888,7 @@ static cudaError_t tile_run(bool prepare, const AttnCall *c, const TileMaps *m, 
   float *parts = reinterpret_cast<float *>(cuts + sms);
   tile_kernel<HD, F16, PAGED><<<sms, TILE_THREADS, tile_smem<HD>(), st>>>(*c, *m, tpt, box, parts, cuts);
   if (cudaError_t e = cudaGetLastError()) return e;
-  return launch_early(join_kernel<HD, F16, TILE_M, 2, 1, 4>, dim3(sms, 2 * TILE_M / (4 * JOIN_WARPS)), 32 * JOIN_WARPS, 0, st, *c,
+  return launch_early(join_kernel<HD, F16, TILE_M, 2, 1, 2>, dim3(sms, 2 * TILE_M / (2 * JOIN_WARPS)), 32 * JOIN_WARPS, 0, st, *c,
                       (const float *)parts, (const AttnCut *)cuts);
 }
 static inline cudaError_t tile_any(bool prepare, int which, const AttnCall *c, const TileMaps *m, int sms, void *ws,

@@ -125,7 +125,7 @@ template <int HD, bool F16, int M, int TILES, int WPR, int RPW>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
 join_kernel(const AttnCall c, const float *__restrict__ parts, const AttnCut *__restrict__ cuts) {
   static_assert(WPR == 1 || RPW == 1, "rows of a warp");
-  constexpr int TF = M * (HD + 2), V = HD / 32, UNROLL = RPW > 1 ? 2 : 4, ROWS = JOIN_WARPS / WPR * RPW;
+  constexpr int TF = M * (HD + 2), V = HD / 32, UNROLL = 4, ROWS = JOIN_WARPS / WPR * RPW;
   __shared__ float s_o[WPR > 1 ? JOIN_WARPS : 1][HD];
   __shared__ float2 s_ml[JOIN_WARPS];
   pdl_wait();
