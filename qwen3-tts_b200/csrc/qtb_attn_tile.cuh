@@ -6,7 +6,7 @@
 // many whole tokens as fit); a block works on two such tiles at a time, against
 // key tiles of 128, in two waves that hide each other:
 //
-//   load warp      Q tiles, then K_0 V_0 K_1 V_1 ... by TMA into a ring (128-byte
+//   load warp      Q tiles, and K_0 V_0 K_1 V_1 ... by TMA into a ring (128-byte
 //                  swizzle; a paged key tile is one box per run of a page's
 //                  positions)
 //   MMA warp       S = Q K^T into tensor memory, and O += P V with P from there;
@@ -25,6 +25,12 @@
 // The probabilities of a tile start from the old maximum at once, beside the new
 // maximum's search, and are thrown away in the rare tile that outgrows it.
 //
+// A pair whose second tile has no token (a decoding request, a short chunk, the
+// end of a prompt) would leave half of the pipeline idle: there both tiles' warps
+// take the same rows, tile 0 every other key tile and tile 1 those between, and
+// their two states are joined in tensor memory at the end ("twin": 64 requests of 8
+// tokens over 4000 keys 199 -> 186 us, a mixed call of 16 requests 152 -> 135).
+//
 // An item of work is a tile pair and a key head.  Where whole items fill the
 // blocks evenly enough (2.5 to a block, or one to at least three of four), they
 // are dealt out whole, longest first.  Where not, the key tiles of all are dealt
@@ -33,7 +39,7 @@
 // costs the parts, the join and the key tiles' reuse in L2, since blocks then walk
 // the keys at as many places as there are blocks (us, whole / cut: 8192-token
 // prompt, 512 items, 212 / 272; 4 x 512 tokens over 8192 keys, 128 items, 122 /
-// 137; 8 x 64 tokens over 8192 keys, 64 items, 133 / 75).
+// 137; 8 x 64 tokens over 8192 keys, 64 items, 129 / 73).
 //
 // What bounds it.  A step (two query tiles, one key tile) needs 2048 cycles of the
 // tensor pipe at 128 dims and 2048 of the MUFU's exponentials, and takes about
@@ -67,8 +73,9 @@ template <int HD>
 constexpr int tile_regs_softmax() { return HD == 128 ? 208 : 200; }
 template <int HD>
 constexpr int tile_regs_other() { return HD == 128 ? 80 : 96; }
-constexpr int TILE_CUT = 1;                // key tiles that a block has of an item at least, where it has not all
-constexpr int TILE_SEGS = 128;             // runs of requests that the in-block search tells apart
+constexpr int TILE_START = 2;              // what starting an item costs, in its steps over a key tile
+constexpr int TILE_CUT = 1;                // steps that a block has of an item at least, where it has not all
+constexpr int TILE_SEGS = 64;              // runs of requests that the in-block search tells apart
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
 template <int HD>
@@ -108,6 +115,7 @@ struct TileShared {
   unsigned char r[TILE_SEGS];
   long long scan[TILE_THREADS / 32];
   int item[2], off[2];                     // the block's first item and place in it, and where the next block's are
+  float2 ml[TILE_M];                       // (m, l) of a twin item's second state
   long long base;                          // units of work before item[1]
 };
 template <int HD>
@@ -246,6 +254,7 @@ struct TileItem {
   int tok0, tok1;       // tokens in each tile
   int from, n0, n1;     // key tiles [from, n0) are this block's for query tile 0, [from, n1) for tile 1
   bool whole;           // those are all
+  bool twin;            // no tile 1: of [from, n0) = [from, n1) tile 0's warps take every other one, tile 1's the rest
   int high;             // keys at and past this are seen by no row
 };
 
@@ -280,7 +289,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     sy.abort = 0;
     fence_mbar_init();
   }
-  // --- pairs of every request, summed over runs of requests: one of the first 128 threads has a run
+  // --- pairs of every request, summed over runs of requests: one of the first TILE_SEGS threads has a run
   const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS;
   auto pairs_of = [&](int n) { return (n + 2 * tpt - 1) / (2 * tpt); };
   int sum = 0, pre = 0;
@@ -359,20 +368,34 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     it.n0 = hi0 > it.low ? (hi0 - it.k0 + TILE_N - 1) / TILE_N : 0;
     it.n1 = it.tok1 > 0 && hi1 > it.low ? (hi1 - it.k0 + TILE_N - 1) / TILE_N : 0;
     it.high = max(hi0, hi1);
+    it.twin = it.tok1 == 0 && it.n0 > 1;
+    if (it.twin) it.n1 = it.n0;
   };
-  // --- this block's run of work.  An item costs its key tiles and one for getting
-  // started; boundaries between blocks move to an item's start or end where less
-  // than TILE_CUT key tiles would be left on that side.
+  // What an item costs, in steps of the two query tiles over a key tile.  A key
+  // tile of a twin item is three quarters of one (it is half of a step, but of one
+  // that loads twice as much): with 1/2, 5/8, 3/4, 7/8, 1 of one a mixed call of 16
+  // requests took 162, 139, 142, 150, 154 us, 8 requests of 64 rows and 8000 keys
+  // 56.0, 56.6, 54.9, 56.5, 54.5; and with TILE_START 1, 2, 3 at 3/4 142, 137, 135
+  // and 54.9, 55.2, 56.4.
+  auto cost_of = [&](const TileItem &it) {
+    const int n = max(it.n0, it.n1);
+    return TILE_START + (it.twin ? (3 * n + 3) >> 2 : n);
+  };
+  auto tiles_at = [&](const TileItem &it, int off) {       // key tiles that cost off past the start
+    return it.twin ? (off - TILE_START) * 4 / 3 : off - TILE_START;
+  };
+  // --- this block's run of work; boundaries between blocks move to an item's start or end where less
+  // than TILE_CUT steps would be left on that side.
   const int items = pairs * c.n_kv;        // the host has bounded it
   const int grid = (int)gridDim.x;
   const bool deal = !parts || tile_whole(items, grid);
   if (deal) {
     if (tid == 0 && parts) cuts[blockIdx.x].last = -1;
   } else {
-    auto cost_of = [&](int p) {
+    auto pair_cost = [&](int p) {
       TileItem it;
       get_pair(p, it);
-      return max(it.n0, it.n1) + 1;
+      return cost_of(it);
     };
     auto scan = [&](long long v, long long &total) {      // inclusive, over the block
       long long x = v;
@@ -392,11 +415,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       }
       return x;
     };
-    int cost = tid < pairs ? cost_of(tid) : 0;
+    int cost = tid < pairs ? pair_cost(tid) : 0;
     long long total, upto = scan(cost, total);
     for (int p0 = TILE_THREADS; p0 < pairs; p0 += TILE_THREADS) {
       long long more;
-      scan(p0 + tid < pairs ? cost_of(p0 + tid) : 0, more);
+      scan(p0 + tid < pairs ? pair_cost(p0 + tid) : 0, more);
       total += more;
     }
     total *= c.n_kv;
@@ -408,7 +431,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     long long before = 0;
     for (int p0 = 0; p0 < pairs; p0 += TILE_THREADS) {
       long long all;
-      if (p0 > 0) cost = p0 + tid < pairs ? cost_of(p0 + tid) : 0;
+      if (p0 > 0) cost = p0 + tid < pairs ? pair_cost(p0 + tid) : 0;
       if (pairs > TILE_THREADS) upto = scan(cost, all);
       __syncthreads();
 #pragma unroll
@@ -417,7 +440,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         const long long x = total * (blockIdx.x + e) / blocks, first = (before + upto - cost) * c.n_kv;
         if (x < first || x >= first + (long long)cost * c.n_kv) continue;
         int h = (int)((unsigned)(x - first) / (unsigned)cost), off = (int)(x - first) - h * cost;
-        if (off < 1 + TILE_CUT) off = 0;
+        if (off < TILE_START + TILE_CUT) off = 0;
         else if (cost - off < TILE_CUT) { off = 0; h++; }
         sh.item[e] = (p0 + tid) * c.n_kv + h;   // h may be n_kv: the next pair's first
         sh.off[e] = off;
@@ -431,7 +454,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       TileItem it;
       if (blockIdx.x < blocks && sh.off[1] > 0 && !(sh.item[0] == sh.item[1] && sh.off[0] > 0)) {
         get_pair(sh.item[1] / c.n_kv, it);
-        const int cost = max(it.n0, it.n1) + 1;
+        const int cost = cost_of(it);
         last = blockIdx.x + 1;
         for (long long x; last + 1 < blocks && (x = total * (last + 1) / blocks - sh.base) < cost && cost - x >= TILE_CUT;) last++;
       }
@@ -451,14 +474,15 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       if (i >= items) return false;
     } else {
       i = sh.item[0] + n;
-      if (n == 0) from = max(sh.off[0] - 1, 0);
+      if (n == 0) from = sh.off[0];
       if (i >= sh.item[1]) off1 = sh.off[1];
       if (i > sh.item[1] || (i == sh.item[1] && off1 == 0)) return false;
     }
     const int p = (int)((unsigned)i / (unsigned)c.n_kv);
     get_pair(deal ? pairs - 1 - p : p, it);
     it.h = i - p * c.n_kv;
-    const int all = max(it.n0, it.n1), to = off1 > 0 ? off1 - 1 : all;
+    const int all = max(it.n0, it.n1), to = off1 > 0 ? tiles_at(it, off1) : all;
+    if (from > 0) from = tiles_at(it, from);
     it.from = from;
     it.whole = from == 0 && to == all;
     it.n0 = max(min(to, it.n0), from);
@@ -499,8 +523,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         n_items++;
         return true;
       };
-#pragma unroll 1
-      for (int j = it.from; j < to && ok; j++) {
+      // K (kv = 0) or V of key tile j into the ring's next place
+      auto load = [&](int kv, int j) {
         const int kb = it.k0 + j * TILE_N;
         // this lane's box of the key tile: positions [pos, pos + box), 64 dims
         const int boxes = PAGED ? TILE_N / box : 1, bi = lane / (HD / 64), x = lane % (HD / 64);
@@ -514,22 +538,29 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
           if (pg < 0 || pg >= c.n_pages) { pg = c.n_pages; bad |= QTB_PS_PAGE; }   // past the last page: reads zeros
         }
         const int count = __popc(__ballot_sync(0xffffffffu, mine));
-#pragma unroll
-        for (int kv = 0; kv < 2; kv++) {
-          const int st = (int)(fill % STAGES);
-          if (!__all_sync(0xffffffffu, wait(&sy.kv_empty[st], ((fill / STAGES) & 1) ^ 1))) { ok = false; break; }
-          if (lane == 0) mbar_arrive_expect_tx(&sy.kv_full[st], (uint32_t)(count * box * 128));
-          __syncwarp();
-          if (mine) {
-            unsigned char *dst = s_kv + st * KV_B + x * HALF_B + bi * box * 128;
-            const CUtensorMap *map = kv ? &maps.v : &maps.k;
-            if (PAGED) tma_load_4d(dst, map, x * 64, off, it.h, pg, &sy.kv_full[st]);
-            else tma_load_4d(dst, map, x * 64, it.t0 + pos, it.h, 0, &sy.kv_full[st]);
-          }
-          fill++;
-          // the queries' buffer may still serve the item before: its keys go first
-          if (kv == 0 && j == it.from && !load_q()) { ok = false; break; }
+        const int st = (int)(fill % STAGES);
+        if (!__all_sync(0xffffffffu, wait(&sy.kv_empty[st], ((fill / STAGES) & 1) ^ 1))) return false;
+        if (lane == 0) mbar_arrive_expect_tx(&sy.kv_full[st], (uint32_t)(count * box * 128));
+        __syncwarp();
+        if (mine) {
+          unsigned char *dst = s_kv + st * KV_B + x * HALF_B + bi * box * 128;
+          const CUtensorMap *map = kv ? &maps.v : &maps.k;
+          if (PAGED) tma_load_4d(dst, map, x * 64, off, it.h, pg, &sy.kv_full[st]);
+          else tma_load_4d(dst, map, x * 64, it.t0 + pos, it.h, 0, &sy.kv_full[st]);
         }
+        fill++;
+        return true;
+      };
+      // in the order in which the MMA warp needs them: K of the first step(s), then V
+      // of a step and K of the next of the same tile.  The queries' buffer may still
+      // serve the item before: its keys go first.
+      const int ahead = it.twin ? 2 : 1;
+      ok = load(0, it.from) && load_q();
+      if (ok && it.twin && it.from + 1 < to) ok = load(0, it.from + 1);
+#pragma unroll 1
+      for (int j = it.from; j < to && ok; j++) {
+        ok = load(1, j);
+        if (ok && j + ahead < to) ok = load(0, j + ahead);
       }
     }
     // copies in flight land before the block leaves
@@ -556,7 +587,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       wait(&sy.q_full, n_items & 1);
       n_items++;
       auto scores = [&](int t, int st) {
-        const uint64_t q = q_desc + (uint32_t)(t * (Q_B >> 4)), k = k_desc + (uint32_t)(st * (KV_B >> 4));
+        const uint64_t q = q_desc + (uint32_t)(it.twin ? 0 : t * (Q_B >> 4)), k = k_desc + (uint32_t)(st * (KV_B >> 4));
         const uint32_t d = tmem + S_COL + t * 128;
         if (elect_one()) {
 #pragma unroll
@@ -568,9 +599,71 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         }
         __syncwarp();
       };
+      // O += P V of key tile in stage sv for tile t, P's second half when it is there;
+      // its K follows in stage sk where there is one
+      auto product = [&](int t, int sv, bool first, bool last) {
+        const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
+        const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = 0; ks < TILE_N / 32; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, !first || ks > 0);
+        }
+        __syncwarp();
+        wait(&sy.p_full[t][1], (p_n >> t) & 1);
+        p_n ^= 1u << t;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int ks = TILE_N / 32; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, 1);
+          if (last) umma_commit(&sy.o_full[t]);
+        }
+        __syncwarp();
+        if (last) o_n ^= 1u << t;
+      };
+      // The first half of P of tile t, and with it V and the next K, the fills f and
+      // f + 1 (lanes wait for one each: the waits' latencies would add up).
+      auto inputs = [&](int t, uint32_t f, bool more, bool first) {
+        uint64_t *bar = &sy.p_full[t][0];
+        uint32_t par = (p_n >> t) & 1;
+        if (lane == 1) { bar = &sy.kv_full[f % STAGES]; par = (f / STAGES) & 1; }
+        if (lane == 2 && more) { bar = &sy.kv_full[(f + 1) % STAGES]; par = ((f + 1) / STAGES) & 1; }
+        if (lane == 3 && first) { bar = &sy.o_empty[t]; par = ((o_n >> t) & 1) ^ 1; }
+        wait(bar, par);
+      };
+      issued = true;
+      if (it.twin) {
+#pragma unroll 1
+        for (int t = 0; t < min(2, to - it.from); t++) {
+          const int st = (int)(fill % STAGES);
+          wait(&sy.kv_full[st], (fill / STAGES) & 1);
+          scores(t, st);
+          if (elect_one()) {
+            umma_commit(&sy.kv_empty[st]);
+            if (t == to - it.from - 1) umma_commit(&sy.q_empty);
+          }
+          __syncwarp();
+          fill++;
+        }
+#pragma unroll 1
+        for (int j = it.from; j < to; j++) {
+          const int t = (j - it.from) & 1, sv = (int)(fill % STAGES), sk = (int)((fill + 1) % STAGES);
+          const bool more = j + 2 < to, first = j < it.from + 2;
+          inputs(t, fill, more, first);
+          product(t, sv, first, !more);
+          if (more) scores(t, sk);
+          if (elect_one()) {
+            umma_commit(&sy.kv_empty[sv]);
+            if (more) umma_commit(&sy.kv_empty[sk]);
+            if (j + 3 == to) umma_commit(&sy.q_empty);
+          }
+          __syncwarp();
+          fill += more ? 2 : 1;
+        }
+        continue;
+      }
       int st = (int)(fill % STAGES);
       wait(&sy.kv_full[st], (fill / STAGES) & 1);
-      issued = true;
       if (it.n0 > it.from) scores(0, st);
       if (it.n1 > it.from) scores(1, st);
       if (elect_one()) {
@@ -587,32 +680,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         for (int t = 0; t < 2; t++) {
           const int n = t ? it.n1 : it.n0;
           if (j >= n) continue;
-          // The first half of P of this tile, and with it V of this step and K of the
-          // next (lanes wait for one each: the waits' latencies would add up).
-          uint64_t *bar = &sy.p_full[t][0];
-          uint32_t par = (p_n >> t) & 1;
-          if (lane == 1) { bar = &sy.kv_full[sv]; par = (fill / STAGES) & 1; }
-          if (lane == 2 && more) { bar = &sy.kv_full[sk]; par = ((fill + 1) / STAGES) & 1; }
-          if (lane == 3 && j == it.from) { bar = &sy.o_empty[t]; par = ((o_n >> t) & 1) ^ 1; }
-          wait(bar, par);
-          tc_fence_after();
-          const uint64_t v = v_desc + (uint32_t)(sv * (KV_B >> 4));
-          const uint32_t d = tmem + O_COL + t * HD, p = tmem + S_COL + t * 128;
-          if (elect_one()) {
-#pragma unroll
-            for (int ks = 0; ks < TILE_N / 32; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, j > it.from || ks > 0);
-          }
-          __syncwarp();
-          wait(&sy.p_full[t][1], (p_n >> t) & 1);
-          p_n ^= 1u << t;
-          tc_fence_after();
-          if (elect_one()) {
-#pragma unroll
-            for (int ks = TILE_N / 32; ks < TILE_N / 16; ks++) umma_ts(d, p + ks * 8, v + ks * (2048 >> 4), idesc_o, 1);
-            if (j == n - 1) umma_commit(&sy.o_full[t]);
-          }
-          __syncwarp();
-          if (j == n - 1) o_n ^= 1u << t;
+          inputs(t, fill, more, j == it.from);
+          product(t, sv, j == it.from, j == n - 1);
           if (j + 1 < n) scores(t, sk);
         }
         if (elect_one()) {
@@ -641,10 +710,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     for (int i = 0;; i++) {
       TileItem it;
       if (!get_item(i, it)) break;
-      const int to = max(it.n0, it.n1), n = t ? it.n1 : it.n0, n_tok = t ? it.tok1 : it.tok0;
+      const int to = max(it.n0, it.n1), n = t ? it.n1 : it.n0, n_tok = t && !it.twin ? it.tok1 : it.tok0;
+      const int tok = it.tok + (it.twin ? 0 : t * tpt), step = it.twin ? 2 : 1, begin = it.from + (it.twin ? t : 0);
       const int tt = row / c.group;
-      const int pos = it.first + it.tok + t * tpt + tt;           // this row's position
-      const int tk = tt < n_tok ? it.t0 + it.tok + t * tpt + tt : -1;   // its packed token (-1: no row)
+      const int pos = it.first + tok + tt;                        // this row's position
+      const int tk = tt < n_tok ? it.t0 + tok + tt : -1;          // its packed token (-1: no row)
       const int head = it.h * c.group + row - tt * c.group;
       // key tiles [clear_a, clear_b) are seen whole by every row of the tile
       const int pos_a = pos - tt, pos_b = pos_a + n_tok - 1;
@@ -653,7 +723,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
       float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-      for (int j = it.from; j < n; j++) {
+      for (int j = begin; j < n; j += step) {
         wait(&sy.s_full[t], s_n & 1);
         s_n++;
         tc_fence_after();
@@ -676,7 +746,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
           }
           if (kb < it.low || kb + TILE_N > it.high) {
             // keys that no row sees: their V may be anything, and 0 * NaN is NaN
-            const uint32_t f = fill + 2 * (j - it.from) + 1;
+            const int v_j = j - it.from;   // V's place among the item's fills
+            const uint32_t f = fill + (it.twin ? 2 + v_j + min(v_j, to - it.from - 2) : 2 * v_j + 1);
             unsigned char *v = s_kv + (f % STAGES) * KV_B;
             wait(&sy.kv_full[f % STAGES], (f / STAGES) & 1);
             if (kb + row < it.low || kb + row >= it.high) {
@@ -728,7 +799,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         // Past the first tile m rarely moves: the probabilities start from the old
         // one while the maximum is taken beside them, and are made anew where a row
         // has outgrown it.
-        bool anew = j == it.from;
+        bool anew = j == begin;
         if (!anew) {
           sum[0] = sum[1] = 0;
 #pragma unroll
@@ -741,7 +812,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
             const float m2 = fmaxf(m, top), f = m2 == -INFINITY ? 1.f : exp2_approx(m - m2);
             m = m2;
             l *= f;
-            if (j > it.from) {
+            if (j > begin) {
 #pragma unroll 1
               for (int x = 0; x < HD / 8; x++) {
                 float o[8];
@@ -767,7 +838,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         l += la + lb;
       }
       fill += 2 * (to - it.from);
-      const bool some = n > it.from;
+      const bool some = n > begin;
       if (some) {
         wait(&sy.o_full[t], o_n & 1);
         o_n++;
@@ -790,7 +861,33 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
             }
           }
       };
-      if (it.whole) {
+      // A twin item's second state reaches the first one's threads: they are in the
+      // same lanes of tensor memory.
+      float f0 = 1.f, f1 = 0.f;
+      if (it.twin) {
+        if (t == 1) {
+          sh.ml[row] = make_float2(m, l);
+          tc_fence_before();
+        }
+        bar_sync_n(1, 256);
+        if (t == 0) {
+          tc_fence_after();
+          const float2 z = sh.ml[row];
+          const float m2 = fmaxf(m, z.x), base = m2 == -INFINITY ? 0.f : m2;
+          f0 = exp2_approx(m - base);
+          f1 = exp2_approx(z.x - base);
+          m = m2;
+          l = l * f0 + z.y * f1;
+        }
+      }
+      const bool both = it.twin && it.from + 1 < n;
+      if (it.twin && t == 1) {
+        // nothing to write: tile 0's warps have both states
+        if (!it.whole) {
+          float *part = parts + ((long long)(2 * blockIdx.x + (it.from == 0 ? 1 : 0)) * 2 + 1) * tile_part_floats<HD>();
+          *reinterpret_cast<float2 *>(part + TILE_M * HD + 2 * row) = make_float2(-INFINITY, 0.f);
+        }
+      } else if (it.whole) {
         const float inv = l > 0.f || l != l ? 1.f / l : 0.f;   // no visible key: zeros
         const long long at = tk >= 0 ? (long long)tk * c.o_st + head * c.o_sh : -1;
         long long rows[4];
@@ -802,6 +899,13 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
           if (some) {
             tmem_ld32_async(o_at + 32 * x, o);
             tmem_ld_wait();
+          }
+          if (both) {
+            float z[32];
+            tmem_ld32_async(o_at + HD + 32 * x, z);
+            tmem_ld_wait();
+#pragma unroll
+            for (int y = 0; y < 32; y++) o[y] = o[y] * f0 + z[y] * f1;
           }
           uint32_t w[4][4];
 #pragma unroll
@@ -825,6 +929,13 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
             uint32_t w[4][4];
             tmem_ld16_async(o_at + 16 * x, reinterpret_cast<float *>(w));
             tmem_ld_wait();
+            if (both) {
+              float z[16];
+              tmem_ld16_async(o_at + HD + 16 * x, z);
+              tmem_ld_wait();
+#pragma unroll
+              for (int y = 0; y < 16; y++) w[y >> 2][y & 3] = __float_as_uint(__uint_as_float(w[y >> 2][y & 3]) * f0 + z[y] * f1);
+            }
             turn(w);
 #pragma unroll
             for (int y = 0; y < 4; y++)
@@ -834,8 +945,9 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         }
         *reinterpret_cast<float2 *>(part + TILE_M * HD + 2 * row) = make_float2(m, l);
       }
+      tc_fence_before();
+      if (it.twin) bar_sync_n(2, 256);     // both states have been read
       if (some) {
-        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&sy.o_empty[t]);
       }

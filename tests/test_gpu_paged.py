@@ -167,6 +167,15 @@ def test_chunks_over_pages(torch, P, heads, kv, d, name, new, kv_len):
     run_paged(torch, P, kv_len, new, heads, kv, d, 16, name, seed=heads + len(new))
 
 
+# One tile of rows over 1 to 5 key tiles, and cut between blocks at odd places; the pages' other positions hold garbage.
+@pytest.mark.parametrize("heads,kv,d,name", [(32, 2, 128, "bf16"), (40, 2, 64, "f16")])
+@pytest.mark.parametrize("kv_len", [[127, 128, 129, 255, 256, 257, 384, 385, 512], [513, 640, 641], [3000, 130, 4001, 7, 1919],
+                                    [2305] * 40])
+@pytest.mark.parametrize("window", [0, 1, 140, 300])
+def test_one_tile_of_rows_over_many_keys(torch, P, heads, kv, d, name, kv_len, window):
+    run_paged(torch, P, kv_len, [3] * len(kv_len), heads, kv, d, 16, name, window=window, seed=len(kv_len) + window)
+
+
 @pytest.mark.parametrize("new,kv_len", [([0, 1, 0, 3, 0], [5, 5, 0, 3, 100]), ([4, 2], [0, 1]), ([200, 1], [150, 0]),
                                         ([40], [0]), ([0, 0, 70], [0, 64, 70])])
 @pytest.mark.parametrize("causal", [True, False])
