@@ -29,17 +29,19 @@
 // end of a prompt) would leave half of the pipeline idle: there both tiles' warps
 // take the same rows, tile 0 every other key tile and tile 1 those between, and
 // their two states are joined in tensor memory at the end ("twin": 64 requests of 8
-// tokens over 4000 keys 199 -> 186 us, a mixed call of 16 requests 152 -> 135).
+// tokens over 4000 keys 199 -> 186 us, a mixed call of 16 requests, cut, 152 -> 135).
 //
 // An item of work is a tile pair and a key head.  Where whole items fill the
-// blocks evenly enough (2.5 to a block, or one to at least three of four), they
-// are dealt out whole, longest first.  Where not, the key tiles of all are dealt
-// out in equal runs, whatever the requests' lengths; an item that is cut between
-// blocks leaves its parts in the workspace, and join_kernel adds them.  Cutting
-// costs the parts, the join and the key tiles' reuse in L2, since blocks then walk
-// the keys at as many places as there are blocks (us, whole / cut: 8192-token
-// prompt, 512 items, 212 / 272; 4 x 512 tokens over 8192 keys, 128 items, 122 /
-// 137; 8 x 64 tokens over 8192 keys, 64 items, 129 / 73).
+// blocks evenly enough, they are dealt out whole, longest first.  Where not, the
+// key tiles of all are dealt out in equal runs, whatever the requests' lengths; an
+// item that is cut between blocks leaves its parts in the workspace, and
+// join_kernel adds them.  Cutting costs the parts, the join and the key tiles'
+// reuse in L2, since blocks then walk the keys at as many places as there are
+// blocks.  Evenly enough: the fullest block has at most 5/4 of the mean and 5 steps
+// (us, whole / cut, at fullest and mean: 16 mixed requests 123 / 134 at 69 and 59;
+// 33 of 1 to 74 tokens 22 / 29 at 10 and 9; 37 of 1 to 3 tokens 15 / 19 at 6 and 2;
+// 16 prompts of 1973 to 7895 147 / 107 at 94 and 54; 8 x 64 tokens over 8192 keys
+// 129 / 73 at 50 and 22; 64 tokens over 2112 keys 37 / 21 at 15 and 1).
 //
 // What bounds it.  A step (two query tiles, one key tile) needs 2048 cycles of the
 // tensor pipe at 128 dims and 2048 of the MUFU's exponentials, and takes about
@@ -100,9 +102,10 @@ struct TileSync {
   int abort;
 };
 
-// Whether `items` fill `grid` blocks evenly enough to be dealt out whole.
-QTB_HOST_DEV bool tile_whole(long long items, int grid) {
-  return 2 * items >= 5 * grid || (items <= grid && 4 * items >= 3 * grid);
+// Whether a single request's `items` fill `sms` blocks evenly enough to be dealt out
+// whole, as its launch sees it; a kernel with a workspace looks at their lengths.
+inline bool tile_whole(long long items, int sms) {
+  return 2 * items >= 5 * sms || (items <= sms && 4 * items >= 3 * sms);
 }
 
 // What lies in shared memory behind the operands (which start it, on 1024 bytes).
@@ -114,8 +117,12 @@ struct TileShared {
   int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS];
   unsigned char r[TILE_SEGS];
   long long scan[TILE_THREADS / 32];
+  int most[TILE_THREADS / 32];
   int item[2], off[2];                     // the block's first item and place in it, and where the next block's are
-  float2 ml[TILE_M];                       // (m, l) of a twin item's second state
+  union {
+    int cost[TILE_THREADS];                // of each pair, while the work is shared out
+    float2 ml[TILE_M];                     // (m, l) of a twin item's second state
+  };
   long long base;                          // units of work before item[1]
 };
 template <int HD>
@@ -384,69 +391,76 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   auto tiles_at = [&](const TileItem &it, int off) {       // key tiles that cost off past the start
     return it.twin ? (off - TILE_START) * 4 / 3 : off - TILE_START;
   };
-  // --- this block's run of work; boundaries between blocks move to an item's start or end where less
-  // than TILE_CUT steps would be left on that side.
   const int items = pairs * c.n_kv;        // the host has bounded it
   const int grid = (int)gridDim.x;
-  const bool deal = !parts || tile_whole(items, grid);
+  // Whole items go from the last pair to the first (longest causal ones first), key
+  // heads inside, and to and fro over the blocks, so that the sums come out alike.
+  auto dealt = [&](int n, int block) { return n * grid + (n & 1 ? grid - 1 - block : block); };
+  // --- whether they are dealt out whole: a thread adds up a block's.  Four to a
+  // block (or more pairs than threads, 2.6 to one) come out alike without.
+  long long total = 0;                     // the cost of all
+  bool deal = !parts || items >= 4 * grid || pairs > TILE_THREADS;
+  if (!deal) {
+    if (tid < pairs) {
+      TileItem it;
+      get_pair(tid, it);
+      sh.cost[tid] = cost_of(it);
+    }
+    __syncthreads();
+    int most = 0;
+#pragma unroll 1
+    for (int b = tid; b < grid; b += TILE_THREADS) {
+      int load = 0;
+#pragma unroll 1
+      for (int n = 0, i; (i = dealt(n, b)) < items; n++) load += sh.cost[pairs - 1 - (int)((unsigned)i / (unsigned)c.n_kv)];
+      total += load;
+      most = max(most, load);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    most = __reduce_max_sync(0xffffffffu, most);
+    if (lane == 0) { sh.scan[warp] = total; sh.most[warp] = most; }
+    __syncthreads();
+    total = 0;
+#pragma unroll 1
+    for (int w = 0; w < TILE_THREADS / 32; w++) { total += sh.scan[w]; most = max(most, sh.most[w]); }
+    deal = 4ll * grid * most <= 5 * total + 20 * grid;
+  }
+  // --- this block's run of work; boundaries between blocks move to an item's start
+  // or end where less than TILE_CUT steps would be left on that side.
   if (deal) {
     if (tid == 0 && parts) cuts[blockIdx.x].last = -1;
   } else {
-    auto pair_cost = [&](int p) {
-      TileItem it;
-      get_pair(p, it);
-      return cost_of(it);
-    };
-    auto scan = [&](long long v, long long &total) {      // inclusive, over the block
-      long long x = v;
+    // the costs of the pairs up to this thread's
+    const int cost = tid < pairs ? sh.cost[tid] : 0;
+    long long upto = cost;
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      __syncthreads();
-      if (lane == 31) sh.scan[warp] = x;
-      __syncthreads();
-      total = 0;
-#pragma unroll
-      for (int w = 0; w < TILE_THREADS / 32; w++) {
-        if (w < warp) x += sh.scan[w];
-        total += sh.scan[w];
-      }
-      return x;
-    };
-    int cost = tid < pairs ? pair_cost(tid) : 0;
-    long long total, upto = scan(cost, total);
-    for (int p0 = TILE_THREADS; p0 < pairs; p0 += TILE_THREADS) {
-      long long more;
-      scan(p0 + tid < pairs ? pair_cost(p0 + tid) : 0, more);
-      total += more;
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
     }
-    total *= c.n_kv;
-    const long long blocks = max(min((long long)gridDim.x, total / (2 * TILE_CUT)), 1ll);
+    __syncthreads();
+    if (lane == 31) sh.scan[warp] = upto;
+    const long long blocks = max(min((long long)grid, total / (2 * TILE_CUT)), 1ll);
     if (tid < 2) {                         // where no boundary is found: past the end
       sh.item[tid] = items;
       sh.off[tid] = 0;
     }
-    long long before = 0;
-    for (int p0 = 0; p0 < pairs; p0 += TILE_THREADS) {
-      long long all;
-      if (p0 > 0) cost = p0 + tid < pairs ? pair_cost(p0 + tid) : 0;
-      if (pairs > TILE_THREADS) upto = scan(cost, all);
-      __syncthreads();
+    __syncthreads();
+#pragma unroll 1
+    for (int w = 0; w < warp; w++) upto += sh.scan[w];
+    const long long first = (upto - cost) * c.n_kv;
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        if (blockIdx.x + e >= blocks) continue;
-        const long long x = total * (blockIdx.x + e) / blocks, first = (before + upto - cost) * c.n_kv;
-        if (x < first || x >= first + (long long)cost * c.n_kv) continue;
-        int h = (int)((unsigned)(x - first) / (unsigned)cost), off = (int)(x - first) - h * cost;
-        if (off < TILE_START + TILE_CUT) off = 0;
-        else if (cost - off < TILE_CUT) { off = 0; h++; }
-        sh.item[e] = (p0 + tid) * c.n_kv + h;   // h may be n_kv: the next pair's first
-        sh.off[e] = off;
-        if (e) sh.base = first + (long long)h * cost;
-      }
-      if (pairs > TILE_THREADS) before += all;
+    for (int e = 0; e < 2; e++) {
+      if (blockIdx.x + e >= blocks) continue;
+      const long long x = total * (blockIdx.x + e) / blocks;
+      if (x < first || x >= first + (long long)cost * c.n_kv) continue;
+      int h = (int)((unsigned)(x - first) / (unsigned)cost), off = (int)(x - first) - h * cost;
+      if (off < TILE_START + TILE_CUT) off = 0;
+      else if (cost - off < TILE_CUT) { off = 0; h++; }
+      sh.item[e] = tid * c.n_kv + h;       // h may be n_kv: the next pair's first
+      sh.off[e] = off;
+      if (e) sh.base = first + (long long)h * cost;
     }
     __syncthreads();
     if (tid == 10 * 32) {                  // an item that this block begins and does not finish
@@ -464,13 +478,11 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   }
 
   // The block's n-th item and its share of the key tiles: [from, n0) for query
-  // tile 0, [from, n1) for tile 1.  False past the end.  Whole items go from the
-  // last pair to the first (longest causal ones first), key heads inside, and to
-  // and fro over the blocks, so that the sums come out alike.
+  // tile 0, [from, n1) for tile 1.  False past the end.
   auto get_item = [&](int n, TileItem &it) {
     int i, from = 0, off1 = 0;
     if (deal) {
-      i = n * grid + (n & 1 ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
+      i = dealt(n, blockIdx.x);
       if (i >= items) return false;
     } else {
       i = sh.item[0] + n;
