@@ -61,6 +61,8 @@
 // run on to their end without waiting (what they then read and write lies within
 // the block's own buffers and outputs).
 #pragma once
+#include <climits>
+
 #include "qtb_paged.cuh"
 
 namespace qtb {
@@ -77,6 +79,7 @@ template <int HD>
 constexpr int tile_regs_other() { return HD == 128 ? 80 : 96; }
 constexpr int TILE_START = 2;              // what starting an item costs, in its steps over a key tile
 constexpr int TILE_CUT = 1;                // steps that a block has of an item at least, where it has not all
+constexpr int TILE_PAIRS = 256;            // pairs whose costs are looked at
 constexpr int TILE_SEGS = 64;              // runs of requests that the in-block search tells apart
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
@@ -120,9 +123,10 @@ struct TileShared {
   int most[TILE_THREADS / 32];
   int item[2], off[2];                     // the block's first item and place in it, and where the next block's are
   union {
-    int cost[TILE_THREADS];                // of each pair, while the work is shared out
+    int cost[TILE_PAIRS];                  // of each pair, while the work is shared out
     float2 ml[TILE_M];                     // (m, l) of a twin item's second state
   };
+  unsigned char order[TILE_PAIRS];         // the pairs by cost, where they are dealt out so
   long long base;                          // units of work before item[1]
 };
 template <int HD>
@@ -393,28 +397,37 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   };
   const int items = pairs * c.n_kv;        // the host has bounded it
   const int grid = (int)gridDim.x;
-  // Whole items go from the last pair to the first (longest causal ones first), key
-  // heads inside, and to and fro over the blocks, so that the sums come out alike.
+  // Whole items go from the costliest pair to the cheapest, key heads inside, and to
+  // and fro over the blocks, so that the sums come out alike.  Pairs whose costs are
+  // not looked at go from the last to the first, a request's longest causal ones first.
   auto dealt = [&](int n, int block) { return n * grid + (n & 1 ? grid - 1 - block : block); };
-  // --- whether they are dealt out whole: a thread adds up a block's.  Four to a
-  // block (or more pairs than threads, 2.6 to one) come out alike without.
+  // --- whether they are dealt out whole: a thread adds up a block's.
+  const bool known = parts && pairs <= TILE_PAIRS;
   long long total = 0;                     // the cost of all
-  bool deal = !parts || items >= 4 * grid || pairs > TILE_THREADS;
-  if (!deal) {
+  bool deal = true;
+  if (known) {
+    int cost = 0;
     if (tid < pairs) {
       TileItem it;
       get_pair(tid, it);
-      sh.cost[tid] = cost_of(it);
+      sh.cost[tid] = cost = cost_of(it);
+    }
+    __syncthreads();
+    if (tid < pairs) {
+      int rank = 0;
+#pragma unroll 4
+      for (int p = 0; p < pairs; p++) rank += sh.cost[p] > cost || (sh.cost[p] == cost && p > tid);
+      sh.order[rank] = (unsigned char)tid;
     }
     __syncthreads();
     int most = 0;
 #pragma unroll 1
     for (int b = tid; b < grid; b += TILE_THREADS) {
-      int load = 0;
+      long long load = 0;
 #pragma unroll 1
-      for (int n = 0, i; (i = dealt(n, b)) < items; n++) load += sh.cost[pairs - 1 - (int)((unsigned)i / (unsigned)c.n_kv)];
+      for (int n = 0, i; (i = dealt(n, b)) < items; n++) load += sh.cost[sh.order[(unsigned)i / (unsigned)c.n_kv]];
       total += load;
-      most = max(most, load);
+      most = max(most, (int)min(load, (long long)INT_MAX));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
@@ -491,7 +504,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       if (i > sh.item[1] || (i == sh.item[1] && off1 == 0)) return false;
     }
     const int p = (int)((unsigned)i / (unsigned)c.n_kv);
-    get_pair(deal ? pairs - 1 - p : p, it);
+    get_pair(!deal ? p : known ? sh.order[p] : pairs - 1 - p, it);
     it.h = i - p * c.n_kv;
     const int all = max(it.n0, it.n1), to = off1 > 0 ? tiles_at(it, off1) : all;
     if (from > 0) from = tiles_at(it, from);

@@ -333,6 +333,21 @@ def test_prompts(torch, P, name, heads, kv, d, new):
             at += n
 
 
+# Prompts whose items are dealt out by what they cost, and some too many or too unlike for that.
+@pytest.mark.parametrize("heads,kv,d,name", [(4, 2, 128, "bf16"), (8, 8, 64, "f16"), (8, 1, 128, "f16")])
+@pytest.mark.parametrize("new", [[700, 30, 1500, 5, 900, 64, 0, 333], [520] * 30, [1, 2000, 3], [600, 1, 513, 7] * 20])
+@pytest.mark.parametrize("window", [0, 200])
+def test_prompts_of_unlike_lengths(torch, P, heads, kv, d, name, new, window):
+    gen = torch.Generator().manual_seed(sum(new) + heads)
+    t = sum(new)
+    q, k, v = (torch.randn(t, h, d, generator=gen).to(kind(torch, name)).cuda() for h in (heads, kv, kv))
+    out, lse = P.prompt_attention(q, k, v, offsets(torch, new), max(new), window=window)
+    at = 0
+    for n in new:
+        check(torch, out[at:at + n], lse[at:at + n], q[at:at + n], k[at:at + n], v[at:at + n], d ** -0.5, True, window, name)
+        at += n
+
+
 def test_long_prompt(torch, P):
     gen = torch.Generator().manual_seed(1)
     n = 4097
