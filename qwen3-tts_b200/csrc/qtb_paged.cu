@@ -343,8 +343,8 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
 // long cache to split.  A mixed call goes to the tiles as a whole: single tokens
 // fill them badly, but their keys stream at the same rate, and a second pair of
 // launches costs more (us, tiles / rows and tiles: 16 requests of up to 7000 keys,
-// every fourth with 400 new tokens, 211 / 236; 64 of 1000, every fourth with 64,
-// 62 / 74; 4 of 500, one with 64, 14 / 26).
+// every fourth with 400 new tokens, 204 / 236; 64 of 1000, every fourth with 64,
+// 64 / 74; 4 of 500, one with 64, 15 / 26).
 struct AttnPlan {
   bool tiles;
   bool cut;                // items may be cut between blocks
