@@ -401,7 +401,9 @@ int qtb_paged_append(const qtb_paged_append_t *d, void *stream);
 /* Attention of each request's new tokens.  Query head h reads key head
  * h / (n_heads / n_kv).  Paged form: K and V are pools [page][head][position]
  * [head_dim], request r's keys 0 .. kv_len[r] - 1 lie in table[r], and its new
- * tokens are its last ones (already appended).  Prompt form: K and V are packed
+ * tokens are its last ones (already appended); a request that outgrew its table
+ * row has the keys of its table_cols * page first positions, and its tokens keep
+ * their positions.  Prompt form: K and V are packed
  * like q ([token][head][head_dim]) and table, kv_len, page are not read.  A
  * token at position p sees keys <= p (causal != 0) and > p - window (window >
  * 0).  out = softmax(scale q.k) v in the type of q; lse = log sum exp(scale

@@ -117,7 +117,7 @@ struct TileShared {
   int pre[TILE_SEGS + 1];                  // query tile pairs before each run of requests
   // the requests themselves, where a run is one: in order of their keys, so that
   // items taken from the last to the first begin with the longest
-  int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS];
+  int t0[TILE_SEGS], n[TILE_SEGS], hi[TILE_SEGS], first[TILE_SEGS];
   unsigned char r[TILE_SEGS];
   long long scan[TILE_THREADS / 32];
   int most[TILE_THREADS / 32];
@@ -259,7 +259,7 @@ QTB_DEV uint64_t add2(uint64_t a, uint64_t b) {
 // One unit of work: 2 tpt tokens (a tile pair) of a request, one key head.
 struct TileItem {
   int r, h, t0, tok;    // request, key head, the request's first packed token, first token of the pair
-  int first, end;       // position of the request's token 0, its keys
+  int first, end, n;    // position of the request's token 0, its keys, its tokens
   int low;              // keys before this are seen by no row of the pair
   int k0;               // first key of key tile 0 (a multiple of 128)
   int tok0, tok1;       // tokens in each tile
@@ -320,7 +320,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       }
     }
     if (tid < c.n_req) {
-      sh.t0[place] = a.t0; sh.n[place] = a.n; sh.hi[place] = a.hi; sh.r[place] = (unsigned char)tid;
+      sh.t0[place] = a.t0; sh.n[place] = a.n; sh.hi[place] = a.hi; sh.first[place] = a.first; sh.r[place] = (unsigned char)tid;
     }
     __syncthreads();
     if (tid < c.n_req) sum = pairs_of(sh.n[tid]);
@@ -362,13 +362,14 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     int n_tok = sh.n[lo];
     it.t0 = sh.t0[lo];
     it.end = sh.hi[lo];
+    it.first = sh.first[lo];
     if (seg > 1) {
       it.r = lo * seg;
       AttnReq a = attn_request<PAGED>(c, it.r);
       for (int q; p >= (q = pairs_of(a.n)); a = attn_request<PAGED>(c, ++it.r)) p -= q;
-      n_tok = a.n; it.t0 = a.t0; it.end = a.hi;
+      n_tok = a.n; it.t0 = a.t0; it.end = a.hi; it.first = a.first;
     }
-    it.first = it.end - n_tok;
+    it.n = n_tok;
     it.tok = p * 2 * tpt;
     it.tok0 = min(n_tok - it.tok, tpt);
     it.tok1 = max(min(n_tok - it.tok - tpt, tpt), 0);
@@ -488,7 +489,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
         for (long long x; last + 1 < blocks && (x = total * (last + 1) / blocks - sh.base) < cost && cost - x >= TILE_CUT;) last++;
       }
       cuts[blockIdx.x] = last < 0 ? AttnCut{-1, 0, 0, 0, 0, 0, {0, 0}}
-                                  : AttnCut{last, it.t0, it.end - it.first, (sh.item[1] % c.n_kv) * c.group, it.tok * c.group, tpt * c.group, {0, 0}};
+                                  : AttnCut{last, it.t0, it.n, (sh.item[1] % c.n_kv) * c.group, it.tok * c.group, tpt * c.group, {0, 0}};
     }
   }
 

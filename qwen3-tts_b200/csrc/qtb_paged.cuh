@@ -33,9 +33,15 @@ struct AttnCall {
 // What a request asks for.  Token i of its n new ones sits at position
 // first + i, sees keys up to there (causal) and none at or before
 // first + i - window (window > 0); keys outside [lo, hi) concern none of them.
+// Over pages the new tokens are the request's last, so that the packed token
+// cu[r + 1] - 1 is at position kv_len - 1, whether or not the table has room for
+// that key (hi) and the packed tensors for that token (t0, n): those that exist
+// keep their positions.  Positions are at most 2^30, as the host bounds the room,
+// and longer lengths are taken as that.
 struct AttnReq {
   int t0, n, first, lo, hi;
 };
+constexpr int POS_MAX = 1 << 30;
 
 template <bool PAGED>
 QTB_DEV AttnReq attn_request(const AttnCall &c, int r) {
@@ -43,10 +49,14 @@ QTB_DEV AttnReq attn_request(const AttnCall &c, int r) {
   a.t0 = min(max(c.cu[r], 0), c.n_tokens);
   const int t1 = min(max(c.cu[r + 1], 0), c.n_tokens);
   a.n = max(t1 - a.t0, 0);
-  const long long room = (long long)c.table_cols * c.page;
-  a.hi = PAGED ? max((int)min((long long)c.kv_len[r], room), 0) : a.n;
-  a.first = a.hi - a.n;
-  a.lo = c.window > 0 ? max(a.first - c.window + 1, 0) : 0;   // positions and windows are below 2^30
+  a.hi = a.n;
+  a.first = 0;
+  if (PAGED) {
+    const int len = min(max(c.kv_len[r], 0), POS_MAX);
+    a.hi = min(len, c.table_cols * c.page);                   // the host has bounded the product
+    a.first = (int)max((long long)len - c.cu[r + 1] + a.t0, -(long long)POS_MAX);   // farther before the keys is as far
+  }
+  a.lo = c.window > 0 ? max(a.first - c.window + 1, 0) : 0;   // positions and windows are at most 2^30
   return a;
 }
 

@@ -563,3 +563,57 @@ def test_requests_served_in_chunks_equal_whole_prompts(torch, P, rows, chunk, pa
     for w in worst:
         for x in w:
             assert float(x) <= 4 * U[name], float(x)
+
+
+# ------------------------------------------- lengths that the tensors do not hold --
+def bounded_cache(torch, gen, room, kv, d, page, name):
+    """Three requests' pages, `room` positions each, full of keys; returns pools, table, K and V."""
+    kp, vp, table, ks = make_cache(torch, gen, [room] * 3, kv, d, page, name)
+    return kp, vp, table[:, :room // page].contiguous(), ks
+
+
+def check_at(torch, out, lse, q, k, v, first, causal, window, name):
+    """Tokens at positions first, first + 1, ..., which may lie past the last key."""
+    d, room = q.shape[2], k.shape[0]
+    for i in range(q.shape[0]):
+        p, s = first + i, slice(i, i + 1)
+        if p < room:
+            n = p + 1 if causal else room
+            low = max(p - window + 1, 0) if window else 0
+        else:
+            n, low = room, min(max(p - window + 1, 0), room) if window else 0
+        # the keys that it sees, all of them
+        check(torch, out[s], lse[s], q[s], k[low:n], v[low:n], d ** -0.5, False, 0, name)
+
+
+# hints: one token at most (the kernel of few rows), or none known
+@pytest.mark.parametrize("hints", [(1, 1), (0, 0)])
+@pytest.mark.parametrize("d,name", [(128, "bf16"), (64, "f16")])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 7), (True, 40), (False, 0), (False, 20)])
+def test_tokens_keep_their_positions_past_the_table(torch, P, hints, d, name, causal, window):
+    """A request that outgrew its row: the tokens that fit have the positions that they were appended at."""
+    gen = torch.Generator().manual_seed(21)
+    room, new, kv_len = 64, [10, 3, 5], [70, 50, 200]
+    kp, vp, table, ks = bounded_cache(torch, gen, room, 2, d, 16, name)
+    q = torch.randn(sum(new), 4, d, generator=gen).to(kind(torch, name)).cuda()
+    out, lse = P.paged_attention(q, kp, vp, table, offsets(torch, new), torch.tensor(kv_len, dtype=torch.int32, device="cuda"),
+                                 *hints, causal=causal, window=window)
+    at = 0
+    for n, end, (k, v) in zip(new, kv_len, ks):
+        k, v = k[:end], v[:end]
+        check_at(torch, out[at:at + n], lse[at:at + n], q[at:at + n], k, v, end - n, causal, window, name)
+        at += n
+
+
+@pytest.mark.parametrize("hints", [(1, 1), (0, 0)])
+def test_tokens_keep_their_positions_where_offsets_leave_the_tokens(torch, P, hints):
+    """Tokens that do not exist, before the first or past the last, take none of the others' positions."""
+    gen = torch.Generator().manual_seed(22)
+    kp, vp, table, ks = bounded_cache(torch, gen, 64, 2, 128, 16, "bf16")
+    q = torch.randn(10, 4, 128, generator=gen).bfloat16().cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for cu, spans in [([0, 5, 15, 15], [(0, 5, 59), (5, 10, 54)]), ([-3, 5, 10, 10], [(0, 5, 59), (5, 10, 59)]),
+                      ([-2, 30, 30, 30], [(0, 10, 34)])]:
+        out, lse = P.paged_attention(q, kp, vp, table, torch.tensor(cu, **i32), torch.tensor([64] * 3, **i32), *hints)
+        for (a, b, first), (k, v) in zip(spans, ks):
+            check_at(torch, out[a:b], lse[a:b], q[a:b], k, v, first, True, 0, "bf16")
