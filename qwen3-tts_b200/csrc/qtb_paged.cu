@@ -81,20 +81,41 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const PlanCall c) {
   for (int base = 0; base < c.n_req; base += PLAN_TILE) {
     int past[PLAN_PER], n[PLAN_PER], need[PLAN_PER];
     long long a = 0, b = 0;
+    bool full = false;
+    auto pages_for = [&](int p, int m) {     // that m tokens behind p cached ones have to take
+      const long long end = min((long long)p + m, cap);
+      if ((long long)p + m > cap) full = true;
+      return (int)max((end + c.page - 1) / c.page - ((long long)p + c.page - 1) / c.page, 0ll);
+    };
 #pragma unroll
     for (int i = 0; i < PLAN_PER; i++) {
       const int r = base + tid * PLAN_PER + i;
       int p = r < c.n_req ? c.past[r] : 0, m = r < c.n_req ? c.fresh[r] : 0;
       if (p < 0 || m < 0) { bad |= QTB_PS_LENGTH; p = max(p, 0); m = max(m, 0); }
       past[i] = p; n[i] = m;
-      const long long end = min((long long)p + m, cap);
-      if ((long long)p + m > cap) bad |= QTB_PS_ROW_FULL;
-      need[i] = (int)max((end + c.page - 1) / c.page - ((long long)p + c.page - 1) / c.page, 0ll);
+      need[i] = pages_for(p, m);
       a += m; b += need[i];
     }
-    const long long mine_a = a, mine_b = b;
+    long long mine_a = a, mine_b = b;
     long long ta, tb;
     scan_pair(a, b, s_w, ta, tb);
+    if (tok + ta > c.max_tokens) {           // the same for the whole block
+      // the tokens past max_tokens are dropped, and take no pages
+      long long at = tok + a - mine_a;
+      b = 0;
+      full = false;
+#pragma unroll
+      for (int i = 0; i < PLAN_PER; i++) {
+        const int m = (int)max(min((long long)n[i], c.max_tokens - at), 0ll);
+        at += n[i];
+        need[i] = pages_for(past[i], m);
+        b += need[i];
+      }
+      mine_b = b;
+      long long x = 0, tx;
+      scan_pair(x, b, s_w, tx, tb);
+    }
+    if (full) bad |= QTB_PS_ROW_FULL;
     a += tok - mine_a; b += pages - mine_b;   // exclusive, from the call's start
 #pragma unroll
     for (int i = 0; i < PLAN_PER; i++) {

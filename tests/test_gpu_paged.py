@@ -617,3 +617,56 @@ def test_tokens_keep_their_positions_where_offsets_leave_the_tokens(torch, P, hi
         out, lse = P.paged_attention(q, kp, vp, table, torch.tensor(cu, **i32), torch.tensor([64] * 3, **i32), *hints)
         for (a, b, first), (k, v) in zip(spans, ks):
             check_at(torch, out[a:b], lse[a:b], q[a:b], k, v, first, True, 0, "bf16")
+
+
+def clipped(new, room):
+    got, left = [], room
+    for n in new:
+        got.append(min(int(n), left))
+        left -= got[-1]
+    return got
+
+
+@pytest.mark.parametrize("requests,page,longest,new_hi,share", [(2, 16, 40, 70, 0.6), (64, 16, 100, 40, 0.0), (64, 16, 100, 40, 0.5),
+                                                                (1024, 16, 90, 33, 0.97), (2500, 32, 200, 3, 0.3),
+                                                                (2500, 32, 200, 3, 0.9)])
+def test_plan_takes_no_pages_for_dropped_tokens(torch, P, requests, page, longest, new_hi, share):
+    rng = np.random.default_rng(requests + page)
+    past, new = rng.integers(0, longest + 1, requests), rng.integers(1, new_hi + 1, requests)
+    cols = -(-(longest + new_hi) // page)
+    used = sum(-(-int(a) // page) for a in past)
+    numbers = rng.permutation(used + int(new.sum()) // page + requests).astype(np.int32)
+    table, at = np.full((requests, cols), -1, np.int32), 0
+    for r, a in enumerate(past):
+        n = -(-int(a) // page)
+        table[r, :n] = numbers[at:at + n]
+        at += n
+    free, room = numbers[used:], int(share * new.sum())
+    want = plain_plan(past, clipped(new, room), table, free, 2, page, room)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    dt, status = torch.from_numpy(table).cuda(), torch.zeros(1, **i32)
+    got = P.plan(torch.tensor(past, **i32), torch.tensor(new, **i32), dt, torch.from_numpy(free).cuda(), page, room,
+                 free_head=torch.tensor([2], **i32), status=status)
+    assert int(status) == P.ROOM
+    assert np.array_equal(dt.cpu().numpy(), want[0])
+    for x, y in zip((got.slot, got.pos, got.req, got.cu_new, got.free_head), (*want[1:5], [want[5]])):
+        assert x.tolist() == list(y)
+    assert np.array_equal(got.kv_len.cpu().numpy(), past + np.array(clipped(new, room)))
+
+
+@pytest.mark.parametrize("what,head,rows", [("room", 4, [[5, 6, 10, 11], [12, 13, -1, -1]]), ("row", 6, [[5, 6, 10, 11], [12, 13, 14, 15]]),
+                                            ("negative", 5, [[10, 11, -1, -1], [12, 13, 14, -1]])])
+def test_plan_counts_the_pages_it_took(torch, P, what, head, rows):
+    i32 = dict(dtype=torch.int32, device="cuda")
+    past, new, room = torch.tensor([20, 0], **i32), torch.tensor([30, 40], **i32), 70
+    table = torch.tensor([[5, 6, -1, -1], [-1] * 4], **i32)
+    if what == "room":
+        room = 50
+    if what == "row":
+        new[1] = 65
+        room = 95
+    if what == "negative":
+        past[0] = -4
+        table[0] = -1
+    got = P.plan(past, new, table, torch.arange(10, 20, **i32), 16, room)
+    assert got.free_head.tolist() == [head] and table.tolist() == rows
