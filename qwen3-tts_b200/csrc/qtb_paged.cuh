@@ -130,10 +130,13 @@ constexpr int JOIN_WARPS = 8;
 // side; a lane has HD / 32 dims of each.  Bounded by the latency of a part's
 // loads for few parts (those of UNROLL parts of all its rows are in flight
 // together), by their bytes for many: 148 cut items of 256 rows are about 40 MB
-// and 14 us.
+// and 14 us.  Its blocks may be up while the grid that writes parts and cuts still
+// runs, so neither is read-only to it: they are not declared const __restrict__,
+// which would let the compiler read them through the read-only path, and ahead of
+// pdl_wait.
 template <int HD, bool F16, int M, int TILES, int WPR, int RPW>
 __global__ void __launch_bounds__(32 * JOIN_WARPS)
-join_kernel(const AttnCall c, const float *__restrict__ parts, const AttnCut *__restrict__ cuts) {
+join_kernel(const AttnCall c, const float *parts, const AttnCut *cuts) {
   static_assert(WPR == 1 || RPW == 1, "rows of a warp");
   constexpr int TF = M * (HD + 2), V = HD / 32, UNROLL = 4, ROWS = JOIN_WARPS / WPR * RPW;
   __shared__ float s_o[WPR > 1 ? JOIN_WARPS : 1][HD];

@@ -670,3 +670,22 @@ def test_plan_counts_the_pages_it_took(torch, P, what, head, rows):
         table[0] = -1
     got = P.plan(past, new, table, torch.arange(10, 20, **i32), 16, room)
     assert got.free_head.tolist() == [head] and table.tolist() == rows
+
+
+def test_workspace_reused_by_calls_in_a_row(torch, P):
+    """Calls that cut their work, one behind the other in the same workspace: each joins its own parts."""
+    gen = torch.Generator().manual_seed(23)
+    kv_len = [3000, 1500]
+    kp, vp, table, _ = make_cache(torch, gen, kv_len, 2, 128, 16, "bf16")
+    lens = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    calls = []
+    for i, new in enumerate([[1, 1], [30, 4], [2, 1], [64, 64]] * 4):
+        q = torch.randn(sum(new), 16, 128, generator=gen).bfloat16().cuda()
+        calls.append((q, kp, vp, table, offsets(torch, new), lens, max(new), 3000))
+    alone = []
+    for a in calls:
+        alone.append(P.paged_attention(*a))
+        torch.cuda.synchronize()
+    for _ in range(5):
+        for (o, z), (a, b) in zip([P.paged_attention(*a) for a in calls], alone):
+            assert torch.equal(o, a) and torch.equal(z, b)
