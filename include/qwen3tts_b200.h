@@ -356,9 +356,11 @@ enum {
 };
 enum {
     QTB_PS_NO_PAGES = 1,    /* the free list ran out: table entry and slots -1       */
-    QTB_PS_ROW_FULL = 2,    /* a request outgrew its table row: its last slots -1    */
+    QTB_PS_ROW_FULL = 2,    /* a request outgrew its table row: its last slots -1; attention: it has the keys
+                               of its first positions                                */
     QTB_PS_ROOM = 4,        /* more than max_tokens new tokens: the rest is dropped  */
-    QTB_PS_LENGTH = 8,      /* a negative length: taken as 0                         */
+    QTB_PS_LENGTH = 8,      /* a negative length: taken as 0; offsets that fall or leave the packed tokens:
+                               tokens that do not exist are not read or written      */
     QTB_PS_PAGE = 16,       /* a page or slot outside the pool: read as zeros, not written */
     QTB_PS_TIMEOUT = 32     /* a wait inside a kernel ran out: outputs are incomplete */
 };

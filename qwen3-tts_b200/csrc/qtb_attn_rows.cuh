@@ -110,10 +110,13 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int box, fl
   RowsCursor<PAGED> cur;
   const int ra = (int)((long long)c.n_req * tid / ROWS_THREADS), rb = (int)((long long)c.n_req * (tid + 1) / ROWS_THREADS);
   long long sum = 0;
+  int wrong = 0;
   for (cur.r = ra; cur.r < rb; cur.r++) {
     cur.load(c);
     sum += cur.units(c);
+    if (blockIdx.x == 0) wrong |= attn_wrong<PAGED>(c, cur.r);
   }
+  raise_status(c.status, wrong);
   long long pre = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {

@@ -303,14 +303,20 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   // --- pairs of every request, summed over runs of requests: one of the first TILE_SEGS threads has a run
   const int seg = (c.n_req + TILE_SEGS - 1) / TILE_SEGS;
   auto pairs_of = [&](int n) { return (n + 2 * tpt - 1) / (2 * tpt); };
-  int sum = 0, pre = 0;
+  int sum = 0, pre = 0, wrong = 0;
   if (seg > 1) {
     if (tid < TILE_SEGS)
-      for (int r = tid * seg; r < min((tid + 1) * seg, c.n_req); r++) sum += pairs_of(attn_request<PAGED>(c, r).n);
+      for (int r = tid * seg; r < min((tid + 1) * seg, c.n_req); r++) {
+        sum += pairs_of(attn_request<PAGED>(c, r).n);
+        if (blockIdx.x == 0) wrong |= attn_wrong<PAGED>(c, r);
+      }
   } else {
     AttnReq a = {};
     int place = tid;
-    if (tid < c.n_req) a = attn_request<PAGED>(c, tid);
+    if (tid < c.n_req) {
+      a = attn_request<PAGED>(c, tid);
+      if (blockIdx.x == 0) wrong = attn_wrong<PAGED>(c, tid);
+    }
     if (c.n_req > 1) {
       if (tid < TILE_SEGS) sh.pre[tid] = a.hi;
       __syncthreads();
@@ -325,6 +331,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     __syncthreads();
     if (tid < c.n_req) sum = pairs_of(sh.n[tid]);
   }
+  raise_status(c.status, wrong);
   if (tid < TILE_SEGS) {
     pre = sum;
 #pragma unroll

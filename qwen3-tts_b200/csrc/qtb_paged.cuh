@@ -60,6 +60,15 @@ QTB_DEV AttnReq attn_request(const AttnCall &c, int r) {
   return a;
 }
 
+// What is wrong with a request's offsets and length (QTB_PS_* bits); the kernels'
+// first block reports it.
+template <bool PAGED>
+QTB_DEV int attn_wrong(const AttnCall &c, int r) {
+  const int a = c.cu[r], b = c.cu[r + 1], len = PAGED ? c.kv_len[r] : 0;
+  return (a < 0 || b < a || b > c.n_tokens || len < 0 ? QTB_PS_LENGTH : 0) |
+         (PAGED && len > c.table_cols * c.page ? QTB_PS_ROW_FULL : 0);
+}
+
 // -------------------------------------------------------- element types ----
 template <bool F16>
 QTB_DEV uint32_t pack2(float lo, float hi) {   // round to nearest even

@@ -31,7 +31,7 @@ import qtts_b200 as Q
 
 NO_PAGES, ROW_FULL, ROOM, LENGTH, PAGE, TIMEOUT = 1, 2, 4, 8, 16, 32
 _STATUS = {NO_PAGES: "the free list ran out", ROW_FULL: "a request outgrew its table row",
-           ROOM: "more new tokens than max_tokens", LENGTH: "a negative length",
+           ROOM: "more new tokens than max_tokens", LENGTH: "a negative length, or offsets that fall or leave the tokens",
            PAGE: "a page or slot outside the pool", TIMEOUT: "a wait inside a kernel ran out"}
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 

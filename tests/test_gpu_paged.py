@@ -689,3 +689,27 @@ def test_workspace_reused_by_calls_in_a_row(torch, P):
     for _ in range(5):
         for (o, z), (a, b) in zip([P.paged_attention(*a) for a in calls], alone):
             assert torch.equal(o, a) and torch.equal(z, b)
+
+
+# ------------------------------------------------------ what the device reports --
+@pytest.mark.parametrize("hints", [(1, 1), (0, 0)])
+@pytest.mark.parametrize("requests", [2, 70])
+@pytest.mark.parametrize("cu,lens,bits", [([0, 5, 10], [64, 65], 2), ([0, 5, 10], [2 ** 31 - 1, 64], 2), ([0, 5, 10], [64, -3], 8),
+                                          ([0, 5, 10 ** 9], [64, 64], 8), ([-5, 5, 10], [64, 64], 8), ([0, 7, 3], [64, 64], 8),
+                                          ([0, 5, 10], [64, 64], 0), ([0, 12, 12], [-1, 70], 10)])
+def test_attention_reports_lengths_out_of_range(torch, P, hints, requests, cu, lens, bits):
+    gen = torch.Generator().manual_seed(24)
+    kp, vp, table, _ = bounded_cache(torch, gen, 64, 2, 128, 16, "bf16")
+    q = torch.randn(10, 4, 128, generator=gen).bfloat16().cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    more = requests - 2              # requests of no token behind them
+    cu, lens = cu + [cu[-1]] * more, lens + [64] * more
+    rows = table[:2].repeat(requests // 2, 1)
+    status = torch.zeros(1, **i32)
+    P.paged_attention(q, kp, vp, rows, torch.tensor(cu, **i32), torch.tensor(lens, **i32), *hints, status=status)
+    assert int(status) == bits
+    wrong = P.LENGTH if min(cu) < 0 or max(cu) > 10 or sorted(cu) != cu else 0     # without lengths of keys
+    for scale in (1.0, -1.0):
+        status.zero_()
+        P.prompt_attention(q, q[:, :2], q[:, :2], torch.tensor(cu, **i32), scale=scale, status=status)
+        assert int(status) == wrong
