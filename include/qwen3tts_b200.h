@@ -360,7 +360,9 @@ enum {
                                of its first positions                                */
     QTB_PS_ROOM = 4,        /* more than max_tokens new tokens: the rest is dropped  */
     QTB_PS_LENGTH = 8,      /* a negative length: taken as 0; offsets that fall or leave the packed tokens:
-                               tokens that do not exist are not read or written      */
+                               tokens that do not exist are not read or written, and
+                               none are where requests that share tokens ask for more
+                               work than can be counted                              */
     QTB_PS_PAGE = 16,       /* a page or slot outside the pool: read as zeros, not written */
     QTB_PS_TIMEOUT = 32     /* a wait inside a kernel ran out: outputs are incomplete */
 };

@@ -35,6 +35,9 @@ namespace qtb {
 
 constexpr int ROWS_WARPS = 4, ROWS_THREADS = 32 * (ROWS_WARPS + 1), ROWS_M = 16, ROWS_CHUNK = 64, ROWS_PER_SM = 2;
 constexpr long long ROWS_WAIT = 4000000000ll;   // cycles: about two seconds
+// Units of work, which a block counts in 32 bits: as many keys as this take a quarter
+// of an hour.  Requests that offsets which fall let share their tokens could ask for more.
+constexpr long long ROWS_UNITS = 1ll << 38;
 
 struct RowsMaps {
   CUtensorMap k, v;
@@ -113,7 +116,7 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int box, fl
   int wrong = 0;
   for (cur.r = ra; cur.r < rb; cur.r++) {
     cur.load(c);
-    sum += cur.units(c);
+    sum = min(sum + cur.units(c), ROWS_UNITS);
     if (blockIdx.x == 0) wrong |= attn_wrong<PAGED>(c, cur.r);
   }
   raise_status(c.status, wrong);
@@ -132,6 +135,10 @@ rows_kernel(const AttnCall c, const __grid_constant__ RowsMaps maps, int box, fl
     total += sh.sum[w];
   }
   pre -= sum;
+  if (total >= ROWS_UNITS) {               // no work
+    if (blockIdx.x == 0 && tid == 0) raise_status(c.status, QTB_PS_LENGTH);
+    total = 0;
+  }
   const long long blocks = min((long long)gridDim.x, total);
   if (tid == 0) cuts[blockIdx.x].last = -1;
   if (blockIdx.x >= blocks) return;

@@ -81,6 +81,7 @@ constexpr int TILE_START = 2;              // what starting an item costs, in it
 constexpr int TILE_CUT = 1;                // steps that a block has of an item at least, where it has not all
 constexpr int TILE_PAIRS = 256;            // pairs whose costs are looked at: as many as shared memory has room for
 constexpr int TILE_SEGS = 64;              // runs of requests that the in-block search tells apart
+constexpr int TILE_RUN = (1 << 25) - 1;    // pairs in a run: more than all of a call can be
 constexpr long long TILE_WAIT = 4000000000ll;   // cycles: about two seconds
 
 template <int HD>
@@ -307,7 +308,7 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
   if (seg > 1) {
     if (tid < TILE_SEGS)
       for (int r = tid * seg; r < min((tid + 1) * seg, c.n_req); r++) {
-        sum += pairs_of(attn_request<PAGED>(c, r).n);
+        sum = min(sum + pairs_of(attn_request<PAGED>(c, r).n), TILE_RUN);
         if (blockIdx.x == 0) wrong |= attn_wrong<PAGED>(c, r);
       }
   } else {
@@ -349,6 +350,8 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
     if (w < warp) before += x;
     pairs += x;
   }
+  // more than requests of tokens of their own can have, as offsets that fall let them: no work
+  if (pairs > c.n_tokens / (2 * tpt) + c.n_req) pairs = 0;
   __syncthreads();
   if (tid < TILE_SEGS) sh.pre[tid] = before + pre - sum;
   if (tid == 0) sh.pre[TILE_SEGS] = pairs;

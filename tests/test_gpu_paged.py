@@ -713,3 +713,34 @@ def test_attention_reports_lengths_out_of_range(torch, P, hints, requests, cu, l
         status.zero_()
         P.prompt_attention(q, q[:, :2], q[:, :2], torch.tensor(cu, **i32), scale=scale, status=status)
         assert int(status) == wrong
+
+
+@pytest.mark.parametrize("requests", [12, 100])
+def test_requests_that_share_tokens_without_end(torch, P, requests):
+    """Offsets that fall let requests have the same tokens; work that could no longer be counted is not begun."""
+    gen = torch.Generator().manual_seed(25)
+    n, d = 10240, 64
+    q, k, v = (torch.randn(n, 1, d, generator=gen).bfloat16().cuda() for _ in range(3))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, n] * 6 + [n] * (requests - 11), **i32)    # six times 40 pairs of tiles, where there are 40
+    status, out = torch.zeros(1, **i32), torch.full_like(q, 7.0)
+    P.prompt_attention(q, k, v, cu, out=out, status=status)
+    assert int(status) == P.LENGTH and bool((out == 7).all())
+    pools = [x.reshape(n // 64, 64, 1, d).transpose(1, 2) for x in (k, v)]
+    table = torch.arange(n // 64, **i32).expand(requests, -1)
+    status.zero_()
+    P.paged_attention(q, *pools, table, cu, torch.full((requests,), n, **i32), out=out, status=status)
+    assert int(status) == P.LENGTH and bool((out == 7).all())
+
+
+@pytest.mark.parametrize("hints", [(1, 1), (0, 0)])
+def test_offsets_that_fall(torch, P, hints):
+    gen = torch.Generator().manual_seed(30)
+    kp, vp, table, ks = bounded_cache(torch, gen, 64, 2, 128, 16, "bf16")
+    q = torch.randn(10, 4, 128, generator=gen).bfloat16().cuda()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    status, out = torch.zeros(1, **i32), torch.full_like(q, 7.0)
+    _, lse = P.paged_attention(q, kp, vp, table, torch.tensor([0, 7, 3, 3], **i32), torch.tensor([64] * 3, **i32), *hints, out=out,
+                               status=status)
+    assert int(status) == P.LENGTH and bool((out[7:] == 7).all())
+    check_at(torch, out[:7], lse[:7], q[:7], *ks[0], 57, True, 0, "bf16")
