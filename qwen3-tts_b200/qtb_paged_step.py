@@ -57,6 +57,13 @@ class PagedCache:
         return self.free.shape[0] - self.taken
 
     def begin(self, new: Sequence[int]) -> Step:
+        """New tokens of each row.  What does not fit is refused here, with nothing changed: the device would cut it."""
+        if len(new) != len(self.length) or min(new, default=0) < 0:
+            raise ValueError(f"new tokens of each of {len(self.length)} rows wanted, got {list(new)}")
+        room = self.table.shape[1] * self.page
+        for r, (a, n) in enumerate(zip(self.length, new)):
+            if a + n > room:
+                raise RuntimeError(f"row {r}: {a} and {n} tokens, room for {room}")
         need = sum(self._pages(a + n) - self._pages(a) for a, n in zip(self.length, new))
         if need > self.pages_left():
             raise RuntimeError(f"{need} pages needed, {self.pages_left()} left")

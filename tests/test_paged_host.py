@@ -114,3 +114,31 @@ def test_status_words():
     P.check_status(torch.zeros(1, dtype=torch.int32))
     with pytest.raises(RuntimeError, match="free list.*pool"):
         P.check_status(torch.tensor([P.NO_PAGES | P.PAGE], dtype=torch.int32))
+
+
+# ------------------------------------------------------------------ a step's cache --
+def cache_on_cpu(lengths=(20, 0, 3), page=16, max_len=64, pages=10):
+    """A cache whose rows have some tokens, as after a step (the operators themselves need a GPU)."""
+    import qtb_paged_step
+    c = qtb_paged_step.PagedCache(1, len(lengths), pages, page, max_len, 1, 64, device="cpu")
+    for r, n in enumerate(lengths):
+        k = -(-n // page)
+        c.table[r, :k] = c.free[c.taken:c.taken + k]
+        c.taken += k
+    c.length, c.head = list(lengths), torch.tensor([c.taken], dtype=torch.int32)
+    return c
+
+
+def state(c):
+    return list(c.length), c.taken, int(c.head), c.free.tolist(), c.table.tolist()
+
+
+@pytest.mark.parametrize("new,error", [([1, 1], ValueError), ([1, 1, 1, 1], ValueError), ([1, -1, 0], ValueError), ([], ValueError),
+                                       ([45, 0, 0], RuntimeError), ([0, 65, 0], RuntimeError), ([1, 0, 2 ** 40], RuntimeError),
+                                       ([44, 64, 61], RuntimeError)])
+def test_steps_that_do_not_fit_are_refused(new, error):
+    c = cache_on_cpu()
+    before = state(c)
+    with pytest.raises(error, match="room for 64|of each of 3 rows|pages needed"):
+        c.begin(new)
+    assert state(c) == before
