@@ -71,7 +71,7 @@ class PagedCache:
         plan = P.plan(past, fresh, self.table, self.free, self.page, sum(new), free_head=self.head, status=self.status)
         self.head, self.taken = plan.free_head, self.taken + need
         self.length = [a + n for a, n in zip(self.length, new)]
-        return Step(plan, sum(new), max(new), max(a for a, n in zip(self.length, new) if n))
+        return Step(plan, sum(new), max(new), max((a for a, n in zip(self.length, new) if n), default=0))
 
     def attend(self, step: Step, layer: int, q, k, v, scale=None, window: int = 0):
         """q [tokens][heads][dim], k and v [tokens][key heads][dim] of the step's new tokens, row by row."""

@@ -744,3 +744,17 @@ def test_offsets_that_fall(torch, P, hints):
                                status=status)
     assert int(status) == P.LENGTH and bool((out[7:] == 7).all())
     check_at(torch, out[:7], lse[:7], q[:7], *ks[0], 57, True, 0, "bf16")
+
+
+# ------------------------------------------------------------------------- steps --
+def test_a_step_without_tokens(torch, P):
+    import qtb_paged_step
+    cache = qtb_paged_step.PagedCache(1, 3, 8, 16, 64, 2, 64)
+    for new in ([0, 0, 0], [5, 0, 1], [0, 0, 0], [1, 1, 0]):
+        step = cache.begin(new)
+        t = sum(new)
+        assert step.tokens == t and step.max_new == max(new)
+        q, k, v = (torch.randn(t, h, 64, device="cuda").bfloat16() for h in (4, 2, 2))
+        assert cache.attend(step, 0, q, k, v).shape == (t, 4, 64)
+    cache.check()
+    assert cache.length == [6, 1, 1] and int(cache.head) == cache.taken == 3
