@@ -82,6 +82,8 @@ class PagedCache:
         return out
 
     def retire(self, rows: Sequence[int]) -> None:
+        if len(set(rows)) < len(rows) or not all(0 <= r < len(self.length) for r in rows):
+            raise ValueError(f"different rows below {len(self.length)} wanted, got {list(rows)}")
         pages = [self.table[r, :self._pages(self.length[r])] for r in rows]
         self.free = torch.cat([self.free[self.taken:], *pages])
         self.head, self.taken = torch.zeros_like(self.head), 0

@@ -142,3 +142,17 @@ def test_steps_that_do_not_fit_are_refused(new, error):
     with pytest.raises(error, match="room for 64|of each of 3 rows|pages needed"):
         c.begin(new)
     assert state(c) == before
+
+
+def test_retired_rows_return_their_pages_once():
+    c = cache_on_cpu()                       # pages 0, 1 | none | 2
+    before = state(c)
+    for rows in ([0, 0], [2, -1], [3], [-1], [0, 1, 0]):
+        with pytest.raises(ValueError, match="rows"):
+            c.retire(rows)
+        assert state(c) == before
+    c.retire([2, 1])
+    assert c.free.tolist() == [3, 4, 5, 6, 7, 8, 9, 2] and c.length == [20, 0, 0] and c.taken == int(c.head) == 0
+    c.retire([0])
+    c.retire([])
+    assert sorted(c.free.tolist()) == list(range(10)) and c.length == [0, 0, 0]
