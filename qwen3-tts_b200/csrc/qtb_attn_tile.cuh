@@ -759,7 +759,10 @@ tile_kernel(const AttnCall c, const __grid_constant__ TileMaps maps, int tpt, in
       const int all_last = min(c.causal ? pos_a : it.end - 1, it.end - 1);
       const int clear_a = c.window > 0 ? (max(pos_b - c.window + 1, 0) - it.k0 + TILE_N - 1) / TILE_N : 0;
       const int clear_b = all_last < it.k0 ? 0 : (all_last + 1 - it.k0) / TILE_N;
-      float m = -INFINITY, l = 0.f;
+      // A row of no token (the next request's queries, or old ones) starts from a
+      // maximum that no score passes: the warp renews m for its own rows alone, so
+      // that a request's results do not depend on what is beside it.
+      float m = tk >= 0 ? -INFINITY : INFINITY, l = 0.f;
 #pragma unroll 1
       for (int j = begin; j < n; j += step) {
         wait(&sy.s_full[t], s_n & 1);

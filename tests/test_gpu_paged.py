@@ -758,3 +758,39 @@ def test_a_step_without_tokens(torch, P):
         assert cache.attend(step, 0, q, k, v).shape == (t, 4, 64)
     cache.check()
     assert cache.length == [6, 1, 1] and int(cache.head) == cache.taken == 3
+
+
+# ------------------------------------------------------------ rows beside others --
+@pytest.mark.parametrize("heads,kv", [(4, 4), (5, 1), (8, 2)])
+@pytest.mark.parametrize("n", [1, 17, 70, 130])
+def test_results_do_not_depend_on_other_requests(torch, P, heads, kv, n):
+    """The rows that a tile has beside a request's own are the next request's, or old ones: they must not move its running
+    maximum, which would round its results differently."""
+    gen = torch.Generator().manual_seed(26)
+    d, more = 128, 200
+    q = torch.randn(n + more, heads, d, generator=gen).bfloat16().cuda()
+    k, v = (torch.randn(n + more, kv, d, generator=gen).bfloat16().cuda() for _ in range(2))
+    cu = offsets(torch, [n, more])
+    want, lse = P.prompt_attention(q, k, v, cu, more)
+    check(torch, want[:n], lse[:n], q[:n], k[:n], v[:n], d ** -0.5, True, 0, "bf16")
+    for mul in (0.0, -3.0, 30.0, 300.0):
+        q2 = q.clone()
+        q2[n:] *= mul
+        out, z = P.prompt_attention(q2, k, v, cu, more)
+        assert torch.equal(out[:n], want[:n]) and torch.equal(z[:n], lse[:n])
+
+
+@pytest.mark.parametrize("name", ["bf16", "f16"])
+def test_results_over_pages_do_not_depend_on_other_requests(torch, P, name):
+    gen = torch.Generator().manual_seed(27)
+    kv_len, new = [700, 300, 900], [9, 100, 3]
+    kp, vp, table, _ = make_cache(torch, gen, kv_len, 2, 128, 16, name)
+    q = torch.randn(sum(new), 10, 128, generator=gen).to(kind(torch, name)).cuda()
+    lens = torch.tensor(kv_len, dtype=torch.int32, device="cuda")
+    want, lse = P.paged_attention(q, kp, vp, table, offsets(torch, new), lens, 100, 900)
+    for mul in (0.0, -3.0, 30.0):
+        q2 = q.clone()
+        q2[9:109] *= mul
+        out, z = P.paged_attention(q2, kp, vp, table, offsets(torch, new), lens, 100, 900)
+        for s in (slice(0, 9), slice(109, 112)):
+            assert torch.equal(out[s], want[s]) and torch.equal(z[s], lse[s])
