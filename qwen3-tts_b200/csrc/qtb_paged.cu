@@ -367,13 +367,15 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
 // every fourth with 400 new tokens, 204 / 236; 64 of 1000, every fourth with 64,
 // 64 / 74; 4 of 500, one with 64, 15 / 26).
 struct AttnPlan {
+  long long rows;          // query rows of a request to a key head, at most (0: not known)
   bool tiles;
   bool cut;                // items may be cut between blocks
   size_t ws;               // bytes of workspace
 };
 AttnPlan attn_plan(const AttnCall &c, const qtb_attn_t *d, bool paged, int sms) {
   AttnPlan p;
-  p.tiles = tile_form(c) && !(paged && d->max_new > 0 && d->max_new * c.group <= ROWS_M);
+  p.rows = (d->max_new < (1 << 30) ? d->max_new : 1 << 30) * c.group;   // max_new may be any number
+  p.tiles = tile_form(c) && !(paged && p.rows > 0 && p.rows <= ROWS_M);
   // no second launch for a few key tiles, nor where one request's items are seen to fill the blocks
   const long long pair = 2 * (TILE_M / c.group), items = (c.n_tokens + pair - 1) / pair * c.n_kv;
   p.cut = p.tiles && !(d->max_kv > 0 && d->max_kv <= 4 * TILE_N) && !(c.n_req == 1 && tile_whole(items, sms));
@@ -403,7 +405,7 @@ int attend(const qtb_attn_t *d, bool paged, void *stream) {
     PAGED_TRY(tile_launch(c, paged, f16, hd, m, dev->sms, p.cut ? d->workspace : nullptr, st));
   } else {
     RowsMaps m;
-    const int max_rows = d->max_new > 0 && d->max_new * c.group < ROWS_M ? (int)d->max_new * c.group : ROWS_M;
+    const int max_rows = p.rows > 0 && p.rows < ROWS_M ? (int)p.rows : ROWS_M;
     if (!rows_maps(c, paged, f16, hd, dev->encode, m)) return qtb_fail(QTB_E_UNSUPPORTED, no_map);
     PAGED_TRY(rows_launch(c, paged, f16, hd, m, dev->sms, max_rows, d->workspace, st));
   }

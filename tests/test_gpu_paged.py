@@ -794,3 +794,17 @@ def test_results_over_pages_do_not_depend_on_other_requests(torch, P, name):
         out, z = P.paged_attention(q2, kp, vp, table, offsets(torch, new), lens, 100, 900)
         for s in (slice(0, 9), slice(109, 112)):
             assert torch.equal(out[s], want[s]) and torch.equal(z[s], lse[s])
+
+
+# --------------------------------------------------------------------- arguments --
+def test_bounds_of_any_size_change_nothing(torch, P):
+    gen = torch.Generator().manual_seed(28)
+    kv_len, new = [600, 64], [1, 3]
+    kp, vp, table, ks = make_cache(torch, gen, kv_len, 2, 128, 16, "bf16")
+    q = torch.randn(4, 8, 128, generator=gen).bfloat16().cuda()
+    for m in [(2 ** 62, 2 ** 62), (2 ** 61 + 1, 600), (2 ** 63 - 1, 2 ** 63 - 1)]:
+        out, lse = P.paged_attention(q, kp, vp, table, offsets(torch, new), torch.tensor(kv_len, dtype=torch.int32, device="cuda"), *m)
+        at = 0
+        for r, n in enumerate(new):
+            check(torch, out[at:at + n], lse[at:at + n], q[at:at + n], *ks[r], 128 ** -0.5, True, 0, "bf16")
+            at += n
