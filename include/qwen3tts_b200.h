@@ -348,7 +348,8 @@ int qtb_attention_noalloc(const float *qkv, int batch, int n_heads, int n_kv, in
  *
  * Every field is 64 bits wide.  Strides are in elements; the innermost dimension
  * is contiguous, no axis of q, k, v or out is expanded (stride 0), and tensor
- * pointers and strides are multiples of 16 bytes. */
+ * pointers and strides are multiples of 16 bytes; of an axis of one the stride
+ * does not matter. */
 enum {
     QTB_T_F32 = 0,
     QTB_T_BF16 = 1,

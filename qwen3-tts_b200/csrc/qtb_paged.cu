@@ -296,9 +296,10 @@ int device_info(const DevInfo **out) {
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
-bool rows16(const int64_t *st, int n, int elem) {
+// Strides of whole 16 bytes; that of an axis of one is never used, and may be any.
+bool rows16(const int64_t *st, const int64_t *ext, int n, int elem) {
   for (int i = 0; i < n; i++)
-    if (st[i] < 0 || st[i] * elem % 16) return false;
+    if (ext[i] > 1 && (st[i] < 0 || st[i] % (16 / elem))) return false;
   return true;
 }
 // Strides that a tensor map can hold: an expanded axis (stride 0) it cannot.
@@ -326,7 +327,10 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
     return qtb_fail(QTB_E_INVALID, "null pointer");
   if (!aligned16(d->q) || !aligned16(d->k) || !aligned16(d->v) || !aligned16(d->out))
     return qtb_fail(QTB_E_INVALID, "q, k, v and out must start on 16 bytes");
-  if (!rows16(d->q_stride, 2, 2) || !rows16(d->k_stride, paged ? 3 : 2, 2) || !rows16(d->v_stride, paged ? 3 : 2, 2) || !rows16(d->out_stride, 2, 2))
+  const int64_t qx[2] = {d->n_tokens, d->n_heads}, px[3] = {d->n_pages, d->n_kv, d->page}, tx[2] = {d->n_tokens, d->n_kv};
+  const int64_t *kx = paged ? px : tx;
+  const int kn = paged ? 3 : 2;
+  if (!rows16(d->q_stride, qx, 2, 2) || !rows16(d->k_stride, kx, kn, 2) || !rows16(d->v_stride, kx, kn, 2) || !rows16(d->out_stride, qx, 2, 2))
     return qtb_fail(QTB_E_INVALID, "strides must be non-negative multiples of 16 bytes");
   if (paged) {
     if (d->page < 16 || d->page % 16 || d->page > 65536) return qtb_fail(QTB_E_INVALID, "page %lld: a multiple of 16", (long long)d->page);
@@ -335,12 +339,8 @@ int attn_call(const qtb_attn_t *d, bool paged, AttnCall &c) {
     if ((d->n_req && !d->kv_len) || (d->n_req && d->table_cols && !d->table) || (d->n_pages && (!d->k || !d->v)))
       return qtb_fail(QTB_E_INVALID, "null pointer");
   }
-  {
-    const int64_t qx[2] = {d->n_tokens, d->n_heads}, px[3] = {d->n_pages, d->n_kv, d->page}, tx[2] = {d->n_tokens, d->n_kv};
-    if (!spread(d->q_stride, qx, 2) || !spread(d->out_stride, qx, 2) || !spread(d->k_stride, paged ? px : tx, paged ? 3 : 2) ||
-        !spread(d->v_stride, paged ? px : tx, paged ? 3 : 2))
-      return qtb_fail(QTB_E_INVALID, "an axis of q, k, v or out is expanded (stride 0)");
-  }
+  if (!spread(d->q_stride, qx, 2) || !spread(d->out_stride, qx, 2) || !spread(d->k_stride, kx, kn) || !spread(d->v_stride, kx, kn))
+    return qtb_fail(QTB_E_INVALID, "an axis of q, k, v or out is expanded (stride 0)");
   c = AttnCall{};
   c.q = static_cast<const uint16_t *>(d->q); c.k = static_cast<const uint16_t *>(d->k); c.v = static_cast<const uint16_t *>(d->v);
   c.out = static_cast<uint16_t *>(d->out); c.lse = d->lse; c.cu = d->cu_new; c.status = d->status;
@@ -453,8 +453,9 @@ extern "C" int qtb_paged_append(const qtb_paged_append_t *d, void *stream) {
   if (!d->n_tokens) return QTB_OK;
   if (!d->k || !d->v || !d->slot || (d->n_pages && (!d->kpool || !d->vpool))) return qtb_fail(QTB_E_INVALID, "null pointer");
   const int es = src32 ? 4 : 2;
-  if (!aligned16(d->k) || !aligned16(d->v) || !aligned16(d->kpool) || !aligned16(d->vpool) || !rows16(d->k_stride, 2, es) ||
-      !rows16(d->v_stride, 2, es) || !rows16(d->kpool_stride, 3, 2) || !rows16(d->vpool_stride, 3, 2))
+  const int64_t sx[2] = {d->n_tokens, d->n_kv}, px[3] = {d->n_pages, d->n_kv, d->page};
+  if (!aligned16(d->k) || !aligned16(d->v) || !aligned16(d->kpool) || !aligned16(d->vpool) || !rows16(d->k_stride, sx, 2, es) ||
+      !rows16(d->v_stride, sx, 2, es) || !rows16(d->kpool_stride, px, 3, 2) || !rows16(d->vpool_stride, px, 3, 2))
     return qtb_fail(QTB_E_INVALID, "pointers and strides must be multiples of 16 bytes");
   const DevInfo *dev;
   if (int rc = device_info(&dev)) return rc;

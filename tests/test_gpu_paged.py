@@ -808,3 +808,22 @@ def test_bounds_of_any_size_change_nothing(torch, P):
         for r, n in enumerate(new):
             check(torch, out[at:at + n], lse[at:at + n], q[at:at + n], *ks[r], 128 ** -0.5, True, 0, "bf16")
             at += n
+
+
+def test_strides_of_single_tokens_and_heads_do_not_matter(torch, P):
+    """A tensor's stride along an axis of one is any number: cut from a wider row, or expanded."""
+    gen = torch.Generator().manual_seed(29)
+    kp, vp, table, ks = make_cache(torch, gen, [300], 1, 128, 16, "bf16")
+    lens, cu = torch.tensor([300], dtype=torch.int32, device="cuda"), offsets(torch, [1])
+    row = torch.randn(1, 6 * 128 + 3, generator=gen).bfloat16().cuda()
+    q, k, v = (row.as_strided((1, n, 128), (row.shape[1], 128 if n > 1 else 3, 1), a * 128) for a, n in ((0, 4), (4, 1), (5, 1)))
+    out, lse = P.paged_attention(q, kp, vp, table, cu, lens, 1, 300)
+    check(torch, out, lse, q, *ks[0], 128 ** -0.5, True, 0, "bf16")
+    out, lse = P.prompt_attention(q, k, v, cu, 1)
+    check(torch, out, lse, q, k, v, 128 ** -0.5, True, 0, "bf16")
+    slot = torch.tensor([299 + 16 * int(table[0, 18]) - 288], device="cuda")
+    odd = [p.as_strided(p.shape, (p.stride(0), 3, p.stride(2), 1)) for p in (kp, vp)]     # one head
+    P.append(k, v, *odd, slot)
+    out, lse = P.paged_attention(q, *odd, table, cu, lens, 1, 300)
+    keys, values = (torch.cat([x[:299], y]) for x, y in zip(ks[0], (k, v)))
+    check(torch, out, lse, q, keys, values, 128 ** -0.5, True, 0, "bf16")

@@ -156,3 +156,18 @@ def test_retired_rows_return_their_pages_once():
     c.retire([0])
     c.retire([])
     assert sorted(c.free.tolist()) == list(range(10)) and c.length == [0, 0, 0]
+
+
+@pytest.mark.parametrize("kw", [dict(tokens=1, qs0=515, os0=3), dict(heads=1, n_kv=1, qs1=1, os1=0, ks1=5, vs1=-7), dict(pages=1, ks0=0, vs0=9)])
+def test_strides_of_an_axis_of_one_are_not_refused(kw):
+    """Such calls go on to the device (where there is one, they are given no token here)."""
+    L = P._lib()
+    rc, said = refusal(L.qtb_paged_attention, attn_desc(**kw, n_req=0), 0)
+    assert rc == 0, said
+
+
+def test_strides_of_other_axes_stay_refused():
+    L = P._lib()
+    for kw in (dict(tokens=1, qs1=12), dict(heads=1, n_kv=1, ks0=4), dict(pages=1, ks2=4)):
+        rc, said = refusal(L.qtb_paged_attention, attn_desc(**kw, n_req=0), 0)
+        assert rc == INVALID and "16 bytes" in said, said
