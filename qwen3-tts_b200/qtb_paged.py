@@ -18,6 +18,10 @@ strides over a contiguous last dimension, so a pool laid out [page][position]
 What the device finds wrong with lengths, pages or slots (QTB_PS_* below) is
 ORed into `status`, an int32 tensor of one element that the caller zeroes and
 reads when it likes; check_status raises for it.
+
+These are operators of serving and have no backward: attention of tensors that
+require a gradient returns results whose backward raises, and what append writes
+into a cache is data.
 """
 from __future__ import annotations
 
@@ -170,6 +174,28 @@ def _results(q, out, lse, status, dev):
     return out, lse
 
 
+class _NoBackward(torch.autograd.Function):
+    """Results that were computed from tensors which require a gradient: asking for it raises."""
+
+    @staticmethod
+    def forward(ctx, out, lse, *inputs):
+        ctx.mark_dirty(out, lse)
+        return out, lse
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("paged operators: attention has no backward")
+
+
+def _wants_gradient(out, lse) -> bool:
+    """Whether a call on tensors that require a gradient is recorded."""
+    if not torch.is_grad_enabled():
+        return False
+    if out is not None or lse is not None:
+        raise RuntimeError("paged operators: out and lse cannot be given where an input requires a gradient (use no_grad)")
+    return True
+
+
 def _attend(fn, pool, dev, q, head, tail, few=False):
     """One attention call with the workspace that calls of its kind have needed so far, and again with what
     qtb_attn_workspace asks for where that is not enough."""
@@ -211,6 +237,7 @@ def paged_attention(q, kpool, vpool, table, cu_new, kv_len, max_new: int = 0, ma
         _refuse(dev, ("q", q, kind if kind in _TYPES else torch.bfloat16, (t, h, d)), ("kpool", kpool, kind, (None, None, None, d)),
                 ("vpool", vpool, kind, tuple(pools)), ("table", table, _i32, (n, None)), ("cu_new", cu_new, _i32, (n + 1,)),
                 ("kv_len", kv_len, _i32, (n,)))
+    grad = (q.requires_grad or kpool.requires_grad or vpool.requires_grad) and _wants_gradient(out, lse)
     out, lse = _results(q, out, lse, status, dev)
     os = out.stride()
     _attend(_lib().qtb_paged_attention, 1, dev, q,
@@ -219,7 +246,7 @@ def paged_attention(q, kpool, vpool, table, cu_new, kv_len, max_new: int = 0, ma
             (qs[0], qs[1], os[0], os[1], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], table.stride(0), cols, page, pages, n, t, h, kv, d,
              max_new, max_kv, _TYPES[kind], causal, window or 0, 1 / math.sqrt(d) if scale is None else scale),
             0 < max_new * h <= 16 * kv)
-    return out, lse
+    return _NoBackward.apply(out, lse, q, kpool, vpool) if grad else (out, lse)
 
 
 def prompt_attention(q, k, v, cu_new, max_new: int = 0, scale=None, causal: bool = True, window: int = 0, out=None,
@@ -236,6 +263,7 @@ def prompt_attention(q, k, v, cu_new, max_new: int = 0, scale=None, causal: bool
             and qs[2] == ks[2] == vs[2] == 1 and cu_new.is_contiguous()):
         _refuse(dev, ("q", q, kind if kind in _TYPES else torch.bfloat16, (t, h, d)), ("k", k, kind, (t, None, d)), ("v", v, kind, (t, kv, d)),
                 ("cu_new", cu_new, _i32, (None,)))
+    grad = (q.requires_grad or k.requires_grad or v.requires_grad) and _wants_gradient(out, lse)
     out, lse = _results(q, out, lse, status, dev)
     os = out.stride()
     _attend(_lib().qtb_prompt_attention, 0, dev, q,
@@ -243,7 +271,7 @@ def prompt_attention(q, k, v, cu_new, max_new: int = 0, scale=None, causal: bool
              0 if status is None else status.data_ptr()),
             (qs[0], qs[1], os[0], os[1], ks[0], ks[1], 0, vs[0], vs[1], 0, 0, 0, 0, 0, n, t, h, kv, d,
              max_new, max_new, _TYPES[kind], causal, window or 0, 1 / math.sqrt(d) if scale is None else scale))
-    return out, lse
+    return _NoBackward.apply(out, lse, q, k, v) if grad else (out, lse)
 
 
 def check_status(status) -> None:

@@ -827,3 +827,25 @@ def test_strides_of_single_tokens_and_heads_do_not_matter(torch, P):
     out, lse = P.paged_attention(q, *odd, table, cu, lens, 1, 300)
     keys, values = (torch.cat([x[:299], y]) for x, y in zip(ks[0], (k, v)))
     check(torch, out, lse, q, keys, values, 128 ** -0.5, True, 0, "bf16")
+
+
+def test_results_that_need_a_gradient_say_that_there_is_none(torch, P):
+    q = torch.randn(5, 4, 64, device="cuda").half().requires_grad_()
+    k, v = (torch.randn(5, 2, 64, device="cuda").half() for _ in range(2))
+    cu = offsets(torch, [5])
+    want, _ = P.prompt_attention(q.detach(), k, v, cu, 5)
+    assert not want.requires_grad
+    out, lse = P.prompt_attention(q, k, v, cu, 5)
+    assert torch.equal(out, want)
+    for x in (out, lse):
+        with pytest.raises(RuntimeError, match="no backward"):
+            x.float().sum().backward()
+    with torch.no_grad():
+        assert not P.prompt_attention(q, k, v, cu, 5)[0].requires_grad
+    pool = torch.zeros(2, 2, 16, 64, device="cuda").half()
+    i32 = dict(dtype=torch.int32, device="cuda")
+    out, _ = P.paged_attention(q, pool, pool, torch.zeros(1, 1, **i32), cu, torch.tensor([5], **i32), 5, 5)
+    with pytest.raises(RuntimeError, match="no backward"):
+        out.float().sum().backward()
+    with pytest.raises(RuntimeError, match="gradient"):
+        P.prompt_attention(q, k, v, cu, 5, out=torch.empty_like(want))
