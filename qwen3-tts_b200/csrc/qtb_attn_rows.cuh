@@ -13,7 +13,7 @@
 // workspace, and join_kernel adds them in block order, so results do not depend
 // on timing.
 //
-// m is renewed lazily, when a score passes it by 2^8: until then the
+// m is renewed lazily, when a score passes it by 8: until then the
 // probabilities are at most 2^8 and the quotient O / l does not care.
 //
 // What bounds it is the stream of K and V.  One warp copies by TMA (a box is a

@@ -19,7 +19,7 @@
 //
 // The running maximum is renewed lazily: with scores in units of log2 (scale *
 // log2 e folded in), p = 2^(s - m) where m is a maximum seen so far, at most
-// 2^8 below the true one, so p <= 2^8 and the sum stays exact to f32 rounding;
+// 8 below the true one, so p <= 2^8 and the sum stays exact to f32 rounding;
 // only when a row outgrows that are its O and l scaled.  The final O / l does
 // not depend on m.
 // The probabilities of a tile start from the old maximum at once, beside the new
@@ -50,9 +50,9 @@
 // not kept (8192 tokens): a quarter of the exponentials by a polynomial on the FMA
 // pipe (-2 to -4 %), two threads to a row (-18 %), P handed over in one piece
 // (-1 %), in three (-11 %).  Measured: a 16384-token prompt, 16 / 8 heads, 128 dims
-// 820 to 960 us by the clock that the power limit leaves (1150 to 1340 TFLOP/s);
-// 8192 tokens 215 to 225 us, of 64 dims, where the exponentials weigh twice, 186
-// us (740 TFLOP/s).  A short call is its start: 64 tokens take 9 us, of which a
+// 835 to 960 us by the clock that the power limit leaves (1150 to 1320 TFLOP/s);
+// 8192 tokens 215 to 225 us, of 64 dims, where the exponentials weigh twice, 188
+// us (730 TFLOP/s).  A short call is its start: 64 tokens take 9 us, of which a
 // launch is 2 and most of the rest code fetched for the first time.
 //
 // Products are issued in order, so the commit that completes S of tile j also
